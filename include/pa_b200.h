@@ -42,8 +42,9 @@ enum {
 
 /* Element types. PA_FP8_E4M3 is the OCP FP8 E4M3 format ("e4m3fn": 1 sign,
  * 4 exponent bits with bias 7, 3 mantissa bits, no infinities, 0x7f / 0xff
- * NaN, largest finite 448); it is accepted only as a decode cache type. */
-enum { PA_F16 = 1, PA_BF16 = 2, PA_F32 = 3, PA_F64 = 4, PA_BOOL = 5, PA_FP8_E4M3 = 6 };
+ * NaN, largest finite 448); it is accepted only as a decode cache type. PA_I8
+ * is a signed byte (codes -127..127), accepted only by the pa_cache_* calls. */
+enum { PA_F16 = 1, PA_BF16 = 2, PA_F32 = 3, PA_F64 = 4, PA_BOOL = 5, PA_FP8_E4M3 = 6, PA_I8 = 7 };
 
 /* Mask kinds: none, boolean keep-mask (1 byte per element, nonzero = keep),
  * additive float mask (type mask_dtype) added to the scaled scores. */
@@ -242,6 +243,126 @@ pa_status pa_decode_kv_fwd(const pa_kv_cache_desc* desc, const void* q, const vo
                            const void* v_cache, const int32_t* block_table,
                            const int32_t* seq_lens, void* out, float* lse, void* workspace,
                            size_t workspace_bytes, void* stream);
+
+/*
+ * Block-scaled cache: a key/value cache laid out as above, in the query's
+ * 16-bit type or in 8 bits (PA_FP8_E4M3 or PA_I8) with one float32 scale for
+ * each block of `scale_block` consecutive keys of a page and head, kept apart
+ * for keys and values. Three calls work on it (no reference counterpart; the
+ * attention is reference.py:139-162 per sequence):
+ *   pa_cache_append  writes new tokens behind each sequence, quantising them;
+ *   pa_cache_decode  attends with one query row per sequence and can add each
+ *                    row's softmax weight to a running array;
+ *   pa_cache_evict   shrinks each sequence to a budget of rows by that array.
+ *
+ * Layout. `cache` describes the pages as for pa_decode_kv_fwd, except that
+ * page_size may be any positive number, kv_dtype may be PA_I8, and k_scale and
+ * v_scale must be 1.0. Key row r of a page and head h uses scale
+ *   scales[page * scale_page_stride + h * scale_head_stride + r / scale_block]
+ * and an element stands for code * scale. Paged: scale_block divides page_size.
+ * 16-bit caches have no scales (pass NULL; the scale_* fields are not read).
+ * Per-row arrays (weights, positions) hold one 4-byte element per row of a
+ * sequence and kv head, at b * row_seq_stride + h * row_head_stride + row; the
+ * row strides are read only where such an array is passed.
+ *
+ * Lengths outside [0, max_seq_len] and block-table entries outside
+ * [0, num_pages) are detected on the device and reported by
+ * pa_device_status() (codes 0x201, 0x202): the rows involved are not written,
+ * and pa_cache_decode reads such rows as zeros.
+ *
+ * All calls are asynchronous on `stream`, allocate nothing when given a
+ * workspace, and can be captured into a CUDA graph. Workspaces of calls that
+ * may overlap on the GPU must be different.
+ */
+typedef struct pa_block_cache_desc {
+  pa_kv_cache_desc cache;
+  int64_t scale_block;       /* keys per scale */
+  int64_t scale_head_stride; /* float elements between kv heads */
+  int64_t scale_page_stride; /* float elements between pages */
+  int64_t row_head_stride;   /* elements between kv heads of a per-row array */
+  int64_t row_seq_stride;    /* elements between sequences of a per-row array */
+} pa_block_cache_desc;
+
+/*
+ * Append new_len tokens (new_lens[b] where that is given, each in
+ * [0, new_len]) behind seq_lens[b] rows of every sequence b. k_new and v_new
+ * are q_dtype; element (b, token t, head h, d) of both is at
+ * b * new_seq_stride + t * new_token_stride + h * new_head_stride + d, with
+ * 16-byte aligned bases and strides that are multiples of 8 elements.
+ *
+ * 8-bit caches: the scale of a block that receives rows becomes
+ *   s' = max(need, s),  need = the least power of two with amax <= qmax * need
+ * over the finite magnitudes of its new rows (qmax 448 or 127; at least
+ * 2^-100), where s is the block's scale if it holds earlier rows of the
+ * sequence and 0 if it holds none. New elements are stored as x / s' and, where
+ * s' > s, the block's earlier codes as code * s / s', all rounded to nearest
+ * even. A power of two keeps x / s' exact, so a code is rounded once, and a
+ * growing scale costs earlier codes at most the bits it shifts out. Infinities
+ * saturate; NaN stays NaN in e4m3 and becomes 0 in int8.
+ *
+ * seq_lens (int32 [batch]) is required. seq_lens + new tokens beyond
+ * max_seq_len is an error of that sequence (code 0x201, nothing of it
+ * written). Optional: weights (float, set to 0 for the new rows), positions
+ * (int32, set to start_positions[b] + t, or to the row where start_positions
+ * is NULL), seq_lens_out (int32 [batch], the new lengths; not the same memory
+ * as seq_lens). Pages that receive rows must belong to one sequence only.
+ */
+pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new, const void* v_new,
+                          int64_t new_len, int64_t new_seq_stride, int64_t new_token_stride,
+                          int64_t new_head_stride, const int32_t* new_lens, void* k_cache,
+                          void* v_cache, float* k_scales, float* v_scales,
+                          const int32_t* block_table, const int32_t* seq_lens, float* weights,
+                          int32_t* positions, const int32_t* start_positions,
+                          int32_t* seq_lens_out, void* stream);
+
+/*
+ * Decode over a block-scaled cache: as pa_decode_kv_fwd (same q, out, lse,
+ * grouped heads, empty sequences, rows past the length never used), with the
+ * scales above. NULL seq_lens means max_seq_len keys everywhere.
+ * `weights` (optional): weights[b][h][j] += the softmax weight of key j, summed
+ * over the query heads of kv head h, for every row j of the sequence.
+ * Scales of rows in use must be finite.
+ */
+pa_status pa_cache_decode_workspace_size(const pa_block_cache_desc* desc, int32_t paged,
+                                         int32_t with_weights, size_t* bytes);
+pa_status pa_cache_decode(const pa_block_cache_desc* desc, const void* q, const void* k_cache,
+                          const void* v_cache, const float* k_scales, const float* v_scales,
+                          const int32_t* block_table, const int32_t* seq_lens, void* out,
+                          float* lse, float* weights, void* workspace, size_t workspace_bytes,
+                          void* stream);
+
+/*
+ * Shrink every (sequence, kv head) to its `budget` best rows. Sequences of at
+ * most `budget` rows stay as they are. Otherwise the rows kept are, in this
+ * order, those with position >= next_positions[b] - recent or < sinks, then
+ * those of the largest weight; ties go to the lowest row, NaN ranks lowest. The
+ * k-th evicted row below `budget` receives the k-th kept row at or above it,
+ * so only those rows move, and rows at or above `budget` are left as they were.
+ * Attention does not depend on the order of rows; `positions` says where a row
+ * came from. In 8-bit caches a block that receives rows is rescaled by the
+ * rule of pa_cache_append, its incoming rows being code * scale of their
+ * source.
+ *
+ * positions NULL: a row's position is its index, and next_positions may be
+ * NULL too (the sequence length). 0 <= recent, 0 <= sinks,
+ * recent + sinks <= budget, budget >= 1.
+ * Outputs: kept (int32, dense [batch][kv_heads][budget]): the row that each
+ * row held before, -1 behind a shorter sequence; seq_lens_out (int32 [batch]):
+ * min(length, budget), not the same memory as seq_lens; weights_out and
+ * positions_out (optional): the per-row arrays in the new order, rows behind
+ * the new length left as they were; they may be weights and positions
+ * themselves. weights must be given. Pages of a sequence that is shrunk must
+ * belong to it alone.
+ */
+pa_status pa_cache_evict_workspace_size(const pa_block_cache_desc* desc, int32_t paged,
+                                        int64_t budget, size_t* bytes);
+pa_status pa_cache_evict(const pa_block_cache_desc* desc, void* k_cache, void* v_cache,
+                         float* k_scales, float* v_scales, const int32_t* block_table,
+                         const int32_t* seq_lens, const float* weights, const int32_t* positions,
+                         const int32_t* next_positions, int64_t budget, int64_t recent,
+                         int64_t sinks, float* weights_out, int32_t* positions_out,
+                         int32_t* seq_lens_out, int32_t* kept, void* workspace,
+                         size_t workspace_bytes, void* stream);
 
 /*
  * Allocation-free variant of pa_decode_fwd. It has no counterpart in the

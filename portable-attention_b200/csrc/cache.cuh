@@ -1,0 +1,123 @@
+// Block-scaled key/value cache: the host-side checks, row addressing and 8-bit
+// codes that the append, decode and evict kernels share.
+#pragma once
+
+#include <cuda_fp8.h>
+
+#include "common.cuh"
+#include "kernels.h"
+
+namespace pa {
+
+// Element kinds of a cache (template parameter of every kernel).
+enum : int { kCacheF16 = 0, kCacheBF16 = 1, kCacheE4M3 = 2, kCacheI8 = 3 };
+
+// What the kernels need of a checked descriptor. Strides are in bytes for the
+// cache and in elements for scales and per-row arrays.
+struct CacheView {
+  int64_t key_stride, head_stride, page_stride;
+  int64_t scale_head, scale_page;
+  int64_t row_head, row_seq;
+  int32_t B, Hq, Hkv, D;
+  int32_t page_size, num_pages, max_pages, scale_block, max_len;
+  int32_t kind;
+  int32_t q_bf16;
+  int32_t paged;
+};
+
+// Which optional parts of a descriptor a call uses.
+struct CacheUse {
+  bool paged;
+  bool rows;    // a per-row array (weights, positions) is passed
+  bool decode;  // queries: head groups and the softmax scale matter
+};
+
+// Checks `d` for a call and fills `v` (csrc/cache_append.cu).
+pa_status check_cache(const pa_block_cache_desc* d, const CacheUse& use, CacheView* v,
+                      const char* who);
+// Checks the cache's pointers: non-null, aligned, scales exactly where they belong.
+pa_status check_cache_ptrs(const CacheView& v, const void* k, const void* v_cache,
+                           const void* k_scales, const void* v_scales, const char* who);
+
+#if defined(__CUDACC__)
+
+__host__ __device__ constexpr bool cache_8bit(int kind) { return kind >= kCacheE4M3; }
+__host__ __device__ constexpr int cache_esz(int kind) { return cache_8bit(kind) ? 1 : 2; }
+
+// Page of row `row` of sequence `b`, or -1 (reported) for an entry outside the cache.
+__device__ __forceinline__ int32_t cache_page(const CacheView& v, const int32_t* table, int b, int row,
+                                              int* status) {
+  if (!table) return b;
+  const int32_t page = table[static_cast<int64_t>(b) * v.max_pages + row / v.page_size];
+  if (page < 0 || page >= v.num_pages) {
+    atomicExch(status, kStatusBadPage);
+    return -1;
+  }
+  return page;
+}
+
+__device__ __forceinline__ int64_t cache_row(const CacheView& v, int32_t page, int h, int at) {
+  return page * v.page_stride + h * v.head_stride + at * v.key_stride;
+}
+
+__device__ __forceinline__ int64_t cache_scale(const CacheView& v, int32_t page, int h, int at) {
+  return page * v.scale_page + h * v.scale_head + at / v.scale_block;
+}
+
+// The least power of two s with amax <= qmax * s, at least 2^-100, by exponent
+// arithmetic: amax = m * 2^e with m in [1, 2), qmax = 1.75 * 2^8 (e4m3) or
+// 1.984375 * 2^6 (int8), both exact.
+template <int KIND>
+__device__ __forceinline__ float cache_need_scale(float amax) {
+  const uint32_t bits = __float_as_uint(amax);
+  int e = static_cast<int>(bits >> 23) - 127;
+  const uint32_t man = bits & 0x7fffffu;
+  constexpr uint32_t top = KIND == kCacheE4M3 ? 0x600000u : 0x7e0000u;  // mantissa of qmax
+  e += (man > top ? 1 : 0) - (KIND == kCacheE4M3 ? 8 : 6);
+  e = e < -100 ? -100 : e;  // also zero and subnormal magnitudes
+  return __uint_as_float(static_cast<uint32_t>(e + 127) << 23);
+}
+
+// Two 8-bit codes (low byte first) as floats.
+template <int KIND>
+__device__ __forceinline__ float2 cache_dec2(uint32_t two) {
+  if (KIND == kCacheE4M3) {
+    const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(two & 0xffffu), __NV_E4M3);
+    return __half22float2(*reinterpret_cast<const __half2*>(&h));
+  }
+  return make_float2(static_cast<float>(static_cast<int8_t>(two & 0xff)),
+                     static_cast<float>(static_cast<int8_t>((two >> 8) & 0xff)));
+}
+
+// Nearest 8-bit codes of two floats, ties to even, saturating (low byte first).
+template <int KIND>
+__device__ __forceinline__ uint32_t cache_enc2(float a, float b) {
+  if (KIND == kCacheE4M3)
+    return __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+  int x = __float2int_rn(a), y = __float2int_rn(b);  // NaN gives 0
+  x = x > 127 ? 127 : (x < -127 ? -127 : x);
+  y = y > 127 ? 127 : (y < -127 ? -127 : y);
+  return static_cast<uint32_t>(x & 0xff) | (static_cast<uint32_t>(y & 0xff) << 8);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 cache_unpack(uint32_t w) {
+  if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+
+// Largest finite magnitude of amax and x (NaN and infinities are passed over).
+__device__ __forceinline__ float cache_amax(float amax, float x) {
+  const float m = fabsf(x);
+  return m < INFINITY ? fmaxf(amax, m) : amax;
+}
+
+__device__ __forceinline__ float warp_max(float x) {
+#pragma unroll
+  for (int o = 16; o; o >>= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+
+#endif  // __CUDACC__
+
+}  // namespace pa

@@ -1,0 +1,307 @@
+// pa_cache_append: write new tokens into a block-scaled cache.
+//
+// For a block of scale_block rows of one (sequence, kv head), with x its new
+// rows and c, s the codes and scale of rows it holds already:
+//   need = 2^ceil(log2(max|x| / qmax)),  s' = max(need, s),
+//   new codes rne(x / s'),  old codes rne(c * s / s') where s' > s.
+// Bytes: each new element is read once (2 bytes) and written once (1 byte); the
+// arithmetic is a few operations per element, so the call is bound by memory,
+// or by latency for a single token per sequence.
+//
+// One warp owns one (sequence, block, kv head, K or V), so a scale has one
+// writer and its rows need no other synchronisation. Lanes take 16-byte pieces
+// (8 elements) of consecutive rows.
+#include <math.h>
+
+#include <cmath>
+#include <string>
+
+#include "cache.cuh"
+
+namespace pa {
+
+pa_status check_cache(const pa_block_cache_desc* d, const CacheUse& use, CacheView* v,
+                      const char* who) {
+  const std::string w = std::string(who) + ": ";
+  if (!d) return fail(PA_ERR_INVALID, w + "null descriptor");
+  const pa_kv_cache_desc& c = d->cache;
+  constexpr int64_t kMax = 0x7fffffffLL;
+  if (c.q_dtype != PA_F16 && c.q_dtype != PA_BF16) return fail(PA_ERR_UNSUPPORTED, w + "q dtype must be fp16 or bf16");
+  if (c.kv_dtype != c.q_dtype && c.kv_dtype != PA_FP8_E4M3 && c.kv_dtype != PA_I8)
+    return fail(PA_ERR_UNSUPPORTED, w + "the cache dtype must be the query's dtype, fp8 e4m3 or int8");
+  if (c.head_dim != 64 && c.head_dim != 128) return fail(PA_ERR_UNSUPPORTED, w + "head dim must be 64 or 128");
+  if (c.batch < 0 || c.batch > 65535 * 1024LL) return fail(PA_ERR_INVALID, w + "batch out of range");
+  if (c.kv_heads < 1 || c.kv_heads > 65535) return fail(PA_ERR_INVALID, w + "kv_heads out of range");
+  if (use.decode) {
+    if (c.q_heads < 1 || c.q_heads % c.kv_heads) return fail(PA_ERR_INVALID, w + "q heads must be a multiple of kv heads");
+    if (c.q_heads / c.kv_heads > 16) return fail(PA_ERR_UNSUPPORTED, w + "at most 16 query heads per key/value head");
+    if (!std::isfinite(c.scale)) return fail(PA_ERR_INVALID, w + "scale must be finite");
+  }
+  if (c.k_scale != 1.f || c.v_scale != 1.f)
+    return fail(PA_ERR_INVALID, w + "k_scale and v_scale must be 1 (the scales are per block)");
+  if (c.max_seq_len < 0 || c.max_seq_len > kMax - 1024) return fail(PA_ERR_UNSUPPORTED, w + "too many keys");
+  if (c.page_size < 1 || c.page_size > kMax) return fail(PA_ERR_INVALID, w + "page_size must be in [1, 2^31)");
+  if (c.num_pages < 1 || c.num_pages > kMax) return fail(PA_ERR_INVALID, w + "num_pages must be in [1, 2^31)");
+  const int esz = c.kv_dtype == PA_FP8_E4M3 || c.kv_dtype == PA_I8 ? 1 : 2;
+  constexpr int64_t kMaxStride = 1LL << 46;
+  if (c.key_stride < c.head_dim || c.head_stride < c.head_dim || c.page_stride < c.head_dim)
+    return fail(PA_ERR_INVALID, w + "cache strides must be at least head_dim");
+  if (c.key_stride > kMaxStride || c.head_stride > kMaxStride || c.page_stride > kMaxStride)
+    return fail(PA_ERR_INVALID, w + "cache strides out of range");
+  if (c.key_stride * esz % 16 || c.head_stride * esz % 16 || c.page_stride * esz % 16)
+    return fail(PA_ERR_INVALID, w + "cache strides must be multiples of 16 bytes");
+  if (use.paged) {
+    if (c.max_pages_per_seq < 0 || c.max_pages_per_seq > kMax) return fail(PA_ERR_INVALID, w + "max_pages_per_seq out of range");
+    if (c.max_pages_per_seq < (c.max_seq_len + c.page_size - 1) / c.page_size)
+      return fail(PA_ERR_INVALID, w + "max_pages_per_seq * page_size must cover max_seq_len");
+  } else {
+    if (c.num_pages < c.batch) return fail(PA_ERR_INVALID, w + "without a block table the cache needs one page per sequence");
+    if (c.page_size < c.max_seq_len) return fail(PA_ERR_INVALID, w + "without a block table page_size must be at least max_seq_len");
+  }
+  if (esz == 1) {
+    if (d->scale_block < 1 || d->scale_block > kMax) return fail(PA_ERR_INVALID, w + "scale_block must be in [1, 2^31)");
+    if (use.paged && c.page_size % d->scale_block) return fail(PA_ERR_INVALID, w + "scale_block must divide page_size");
+    const int64_t blocks = (c.page_size + d->scale_block - 1) / d->scale_block;
+    if (d->scale_head_stride < blocks || d->scale_page_stride < blocks)
+      return fail(PA_ERR_INVALID, w + "scale strides must be at least the blocks of a page");
+    if (d->scale_head_stride > kMaxStride || d->scale_page_stride > kMaxStride)
+      return fail(PA_ERR_INVALID, w + "scale strides out of range");
+  }
+  if (use.rows) {
+    if (d->row_head_stride < c.max_seq_len || d->row_seq_stride < c.max_seq_len)
+      return fail(PA_ERR_INVALID, w + "row strides must be at least max_seq_len");
+    if (d->row_head_stride > kMaxStride || d->row_seq_stride > kMaxStride)
+      return fail(PA_ERR_INVALID, w + "row strides out of range");
+  }
+  *v = CacheView{};
+  v->key_stride = c.key_stride * esz;
+  v->head_stride = c.head_stride * esz;
+  v->page_stride = c.page_stride * esz;
+  v->scale_head = d->scale_head_stride;
+  v->scale_page = d->scale_page_stride;
+  v->row_head = d->row_head_stride;
+  v->row_seq = d->row_seq_stride;
+  v->B = static_cast<int32_t>(c.batch);
+  v->Hq = use.decode ? static_cast<int32_t>(c.q_heads) : 0;
+  v->Hkv = static_cast<int32_t>(c.kv_heads);
+  v->D = static_cast<int32_t>(c.head_dim);
+  v->page_size = static_cast<int32_t>(c.page_size);
+  v->num_pages = static_cast<int32_t>(c.num_pages);
+  v->max_pages = use.paged ? static_cast<int32_t>(c.max_pages_per_seq) : 1;
+  v->scale_block = esz == 1 ? static_cast<int32_t>(d->scale_block) : 0;
+  v->max_len = static_cast<int32_t>(c.max_seq_len);
+  v->q_bf16 = c.q_dtype == PA_BF16;
+  v->kind = c.kv_dtype == PA_FP8_E4M3 ? kCacheE4M3 : c.kv_dtype == PA_I8 ? kCacheI8 : v->q_bf16 ? kCacheBF16 : kCacheF16;
+  v->paged = use.paged;
+  return PA_OK;
+}
+
+pa_status check_cache_ptrs(const CacheView& v, const void* k, const void* vc, const void* ks,
+                           const void* vs, const char* who) {
+  const std::string w = std::string(who) + ": ";
+  if (!k || !vc) return fail(PA_ERR_INVALID, w + "null cache pointer");
+  if ((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(vc)) & 15)
+    return fail(PA_ERR_INVALID, w + "cache pointers must be 16-byte aligned");
+  if (cache_8bit(v.kind) && (!ks || !vs)) return fail(PA_ERR_INVALID, w + "8-bit caches need k_scales and v_scales");
+  if (!cache_8bit(v.kind) && (ks || vs)) return fail(PA_ERR_INVALID, w + "16-bit caches have no scales");
+  return PA_OK;
+}
+
+namespace {
+
+struct AppendArgs {
+  CacheView c;
+  const uint8_t* x[2];  // new keys, new values
+  uint8_t* cache[2];
+  float* scales[2];
+  const int32_t* table;
+  const int32_t* lens;
+  const int32_t* new_lens;
+  const int32_t* start;
+  float* weights;
+  int32_t* positions;
+  int32_t* lens_out;
+  int* status;
+  int64_t x_seq, x_tok, x_head;  // bytes
+  int32_t T, blocks, rows_per_block;
+  int64_t items;
+};
+
+template <int KIND, int D, bool QBF16>
+__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+  const int lane = threadIdx.x & 31;
+  const int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
+  if (item >= a.items) return;
+  // Heads vary fastest: token-major inputs and caches hold a token's heads side by side.
+  const int h = static_cast<int>(item % a.c.Hkv);
+  int64_t rest = item / a.c.Hkv;
+  const int kv = static_cast<int>(rest & 1);
+  rest >>= 1;
+  const int blk = static_cast<int>(rest % a.blocks);
+  const int b = static_cast<int>(rest / a.blocks);
+
+  const int len = a.lens[b];
+  int add = a.new_lens ? a.new_lens[b] : a.T;
+  if (len < 0 || len > a.c.max_len || add < 0 || add > a.T || add > a.c.max_len - len) {
+    if (lane == 0) atomicExch(a.status, kStatusBadSeqLen);
+    add = 0;
+  }
+  if (a.lens_out && h == 0 && kv == 0 && blk == 0 && lane == 0) a.lens_out[b] = len + add;
+  const int bs = a.rows_per_block;
+  const int64_t r_first = (static_cast<int64_t>(len / bs) + blk) * bs;  // first row of this block
+  if (add == 0 || r_first >= static_cast<int64_t>(len) + add) return;
+  const int r0 = static_cast<int>(r_first);
+  const int lo = r0 > len ? r0 : len;  // first new row
+  const int hi = static_cast<int>(r_first + bs < static_cast<int64_t>(len) + add ? r_first + bs : len + add);
+
+  if (kv == 0 && (a.weights || a.positions)) {
+    const int64_t row0 = b * a.c.row_seq + h * a.c.row_head;
+    const int p0 = a.start ? a.start[b] : len;
+    for (int r = lo + lane; r < hi; r += 32) {
+      if (a.weights) a.weights[row0 + r] = 0.f;
+      if (a.positions) a.positions[row0 + r] = p0 + (r - len);
+    }
+  }
+  constexpr int kChunks = D / 8;  // 16-byte pieces of a new row
+  const uint8_t* src = a.x[kv] + b * a.x_seq + h * a.x_head;
+  const int n = (hi - lo) * kChunks;
+
+  if (!cache_8bit(KIND)) {
+    for (int i = lane; i < n; i += 32) {
+      const int r = lo + i / kChunks, ch = i % kChunks;
+      const int32_t page = cache_page(a.c, a.table, b, r, a.status);
+      if (page < 0) continue;
+      const uint4 w = *reinterpret_cast<const uint4*>(src + (r - len) * a.x_tok + ch * 16);
+      *reinterpret_cast<uint4*>(a.cache[kv] + cache_row(a.c, page, h, a.table ? r % a.c.page_size : r) + ch * 16) = w;
+    }
+    return;
+  }
+  // 8 bits: the block lies in one page.
+  const int32_t page = cache_page(a.c, a.table, b, lo, a.status);
+  if (page < 0) return;
+  const int at0 = a.table ? r0 % a.c.page_size : r0;  // the block's first row inside its page
+  float amax = 0.f;
+  for (int i = lane; i < n; i += 32) {
+    const uint4 w = *reinterpret_cast<const uint4*>(src + (lo + i / kChunks - len) * a.x_tok + (i % kChunks) * 16);
+    const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = cache_unpack<QBF16>(wd[k]);
+      amax = cache_amax(cache_amax(amax, f.x), f.y);
+    }
+  }
+  amax = warp_max(amax);
+  float* sp = a.scales[kv] + cache_scale(a.c, page, h, at0);
+  const bool held = r0 < len;  // earlier rows of this sequence live in the block
+  const float need = cache_need_scale<KIND>(amax);
+  const float old = held ? *sp : 0.f;
+  const float s = old > need ? old : need;
+  uint8_t* dst = a.cache[kv] + cache_row(a.c, page, h, at0);
+  for (int i = lane; i < n; i += 32) {
+    const int r = lo + i / kChunks, ch = i % kChunks;
+    const uint4 w = *reinterpret_cast<const uint4*>(src + (r - len) * a.x_tok + ch * 16);
+    const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+    uint32_t o[2] = {0u, 0u};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = cache_unpack<QBF16>(wd[k]);
+      o[k >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s)) << (16 * (k & 1));
+    }
+    *reinterpret_cast<uint2*>(dst + (r - r0) * a.c.key_stride + ch * 8) = make_uint2(o[0], o[1]);
+  }
+  if (held && s != old) {
+    // The scale grew: the block's earlier rows are coded again.
+    for (int i = lane; i < (len - r0) * kChunks; i += 32) {
+      uint2* p = reinterpret_cast<uint2*>(dst + (i / kChunks) * a.c.key_stride + (i % kChunks) * 8);
+      const uint2 w = *p;
+      const uint32_t wd[2] = {w.x, w.y};
+      uint32_t o[2] = {0u, 0u};
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float2 f = cache_dec2<KIND>(wd[k >> 1] >> (16 * (k & 1)));
+        o[k >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x * old, s), __fdiv_rn(f.y * old, s)) << (16 * (k & 1));
+      }
+      *p = make_uint2(o[0], o[1]);
+    }
+  }
+  __syncwarp();  // every lane has read the old scale
+  if (lane == 0) *sp = s;
+}
+
+template <int KIND, int D, bool QBF16>
+pa_status launch_append(const AppendArgs& a, cudaStream_t st) {
+  const int64_t grid = (a.items + 7) / 8;
+  if (grid > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache append: grid too large");
+  cache_append_kernel<KIND, D, QBF16><<<static_cast<unsigned>(grid), 256, 0, st>>>(a);
+  PA_CUDA(cudaGetLastError());
+  return PA_OK;
+}
+
+template <int D>
+pa_status launch_append_kind(const AppendArgs& a, cudaStream_t st) {
+  switch (a.c.kind) {
+    case kCacheF16: return launch_append<kCacheF16, D, false>(a, st);
+    case kCacheBF16: return launch_append<kCacheBF16, D, true>(a, st);
+    case kCacheE4M3:
+      return a.c.q_bf16 ? launch_append<kCacheE4M3, D, true>(a, st) : launch_append<kCacheE4M3, D, false>(a, st);
+    default:
+      return a.c.q_bf16 ? launch_append<kCacheI8, D, true>(a, st) : launch_append<kCacheI8, D, false>(a, st);
+  }
+}
+
+}  // namespace
+}  // namespace pa
+
+using namespace pa;
+
+extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new,
+                                     const void* v_new, int64_t new_len, int64_t new_seq_stride,
+                                     int64_t new_token_stride, int64_t new_head_stride,
+                                     const int32_t* new_lens, void* k_cache, void* v_cache,
+                                     float* k_scales, float* v_scales, const int32_t* block_table,
+                                     const int32_t* seq_lens, float* weights, int32_t* positions,
+                                     const int32_t* start_positions, int32_t* seq_lens_out,
+                                     void* stream) {
+  clear_error();
+  AppendArgs a{};
+  PA_TRY(check_cache(desc, {block_table != nullptr, weights || positions, false}, &a.c, "cache append"));
+  if (new_len < 0 || new_len > a.c.max_len) return fail(PA_ERR_INVALID, "cache append: new_len must be in [0, max_seq_len]");
+  if (start_positions && !positions) return fail(PA_ERR_INVALID, "cache append: start_positions without positions");
+  if (a.c.B == 0) return PA_OK;
+  if (!seq_lens) return fail(PA_ERR_INVALID, "cache append: null seq_lens");
+  if (seq_lens_out == seq_lens) return fail(PA_ERR_INVALID, "cache append: seq_lens_out must not be seq_lens");
+  if (new_len > 0) {
+    PA_TRY(check_cache_ptrs(a.c, k_cache, v_cache, k_scales, v_scales, "cache append"));
+    if (!k_new || !v_new) return fail(PA_ERR_INVALID, "cache append: null k_new or v_new");
+    if ((reinterpret_cast<uintptr_t>(k_new) | reinterpret_cast<uintptr_t>(v_new)) & 15)
+      return fail(PA_ERR_INVALID, "cache append: k_new and v_new must be 16-byte aligned");
+    for (int64_t s : {new_seq_stride, new_token_stride, new_head_stride})
+      if (s < 0 || s > (1LL << 46) || s % 8)
+        return fail(PA_ERR_INVALID, "cache append: strides of the new tokens must be non-negative multiples of 8 elements");
+  }
+  a.x[0] = static_cast<const uint8_t*>(k_new);
+  a.x[1] = static_cast<const uint8_t*>(v_new);
+  a.cache[0] = static_cast<uint8_t*>(k_cache);
+  a.cache[1] = static_cast<uint8_t*>(v_cache);
+  a.scales[0] = k_scales;
+  a.scales[1] = v_scales;
+  a.table = block_table;
+  a.lens = seq_lens;
+  a.new_lens = new_lens;
+  a.start = start_positions;
+  a.weights = weights;
+  a.positions = positions;
+  a.lens_out = seq_lens_out;
+  a.status = device_status_word();
+  if (!a.status) return fail(PA_ERR_CUDA, "device status word unavailable");
+  a.x_seq = new_seq_stride * 2;
+  a.x_tok = new_token_stride * 2;
+  a.x_head = new_head_stride * 2;
+  a.T = static_cast<int32_t>(new_len);
+  // 16-bit caches have no blocks: 16 rows make an item.
+  a.rows_per_block = cache_8bit(a.c.kind) ? a.c.scale_block : 16;
+  a.blocks = a.T / a.rows_per_block + 2;  // blocks that T rows starting anywhere can touch
+  a.items = static_cast<int64_t>(a.c.B) * a.blocks * 2 * a.c.Hkv;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  return a.c.D == 128 ? launch_append_kind<128>(a, st) : launch_append_kind<64>(a, st);
+}

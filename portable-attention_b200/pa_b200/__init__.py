@@ -18,6 +18,9 @@ from __future__ import annotations
 
 from ._lib import LibraryError, PaError, library_path
 from .autograd import forward_with_lse, sdpa_backward
+from .blockcache import (AppendResult, EvictResult, block_cache_desc, cache_append, cache_append_device,
+                         cache_decode, cache_decode_device, cache_decode_workspace_size, cache_evict,
+                         cache_evict_device, cache_evict_workspace_size)
 from .backend import scaled_dot_product_attention, sdpa_device, sdpa_sharded
 from .kvcache import decode_kv_cache, decode_kv_device, kv_cache_desc
 from .device import (DeviceBuffer, Event, Stream, current_device, device_count, pinned_empty,
@@ -26,8 +29,10 @@ from .plan import compute_dtype, plan_call
 from .tiling import B200_LIMITS, plan_tcgen05_tiles
 
 __all__ = [
-    "B200_LIMITS", "DeviceBuffer", "Event", "LibraryError", "PaError", "Stream", "available", "compute_dtype",
-    "current_device", "decode_kv_cache", "decode_kv_device", "device_count", "forward_with_lse",
+    "AppendResult", "B200_LIMITS", "DeviceBuffer", "Event", "EvictResult", "LibraryError", "PaError", "Stream",
+    "available", "block_cache_desc", "cache_append", "cache_append_device", "cache_decode", "cache_decode_device",
+    "cache_decode_workspace_size", "cache_evict", "cache_evict_device", "cache_evict_workspace_size",
+    "compute_dtype", "current_device", "decode_kv_cache", "decode_kv_device", "device_count", "forward_with_lse",
     "kv_cache_desc", "library_path", "plan_tcgen05_tiles", "pinned_empty",
     "plan_call", "register", "scaled_dot_product_attention", "sdpa_backward", "sdpa_device", "sdpa_sharded",
     "set_device", "sync_device_status",

@@ -13,13 +13,13 @@ import threading
 from pathlib import Path
 
 __all__ = [
-    "PA_BF16", "PA_BOOL", "PA_F16", "PA_F32", "PA_F64", "PA_FP8_E4M3", "PA_MASK_ADD",
-    "PA_MASK_BOOL", "PA_MASK_NONE", "PA_MAX_LEAD", "KvCacheDesc", "LibraryError", "PaError",
-    "SdpaDesc", "check", "lib", "library_path",
+    "PA_BF16", "PA_BOOL", "PA_F16", "PA_F32", "PA_F64", "PA_FP8_E4M3", "PA_I8", "PA_MASK_ADD",
+    "PA_MASK_BOOL", "PA_MASK_NONE", "PA_MAX_LEAD", "BlockCacheDesc", "KvCacheDesc", "LibraryError",
+    "PaError", "SdpaDesc", "check", "lib", "library_path",
 ]
 
 PA_OK, PA_ERR_INVALID, PA_ERR_UNSUPPORTED, PA_ERR_CUDA, PA_ERR_TIMEOUT, PA_ERR_NCCL, PA_ERR_NOMEM = range(7)
-PA_F16, PA_BF16, PA_F32, PA_F64, PA_BOOL, PA_FP8_E4M3 = 1, 2, 3, 4, 5, 6
+PA_F16, PA_BF16, PA_F32, PA_F64, PA_BOOL, PA_FP8_E4M3, PA_I8 = 1, 2, 3, 4, 5, 6, 7
 PA_MASK_NONE, PA_MASK_BOOL, PA_MASK_ADD = 0, 1, 2
 PA_MAX_LEAD = 6
 
@@ -98,9 +98,25 @@ class KvCacheDesc(ctypes.Structure):
     ]
 
 
+class BlockCacheDesc(ctypes.Structure):
+    """Mirror of ``pa_block_cache_desc`` (include/pa_b200.h)."""
+
+    _fields_ = [
+        ("cache", KvCacheDesc),
+        ("scale_block", ctypes.c_int64),
+        ("scale_head_stride", ctypes.c_int64),
+        ("scale_page_stride", ctypes.c_int64),
+        ("row_head_stride", ctypes.c_int64),
+        ("row_seq_stride", ctypes.c_int64),
+    ]
+
+
 _P = ctypes.c_void_p
 _I32 = ctypes.c_int32
 _DESC = ctypes.POINTER(SdpaDesc)
+_I64 = ctypes.c_int64
+_SIZE = ctypes.c_size_t
+_BC = ctypes.POINTER(BlockCacheDesc)
 _F32P = ctypes.POINTER(ctypes.c_float)
 
 # name -> argtypes; every symbol returns pa_status (int32) unless listed in _RESTYPES.
@@ -136,6 +152,11 @@ SIGNATURES = {
     "pa_decode_fwd_static": [_DESC, _P, _P, _P, _P, _P, _P, _P],
     "pa_decode_kv_workspace_size": [ctypes.POINTER(KvCacheDesc), _I32, ctypes.POINTER(ctypes.c_size_t)],
     "pa_decode_kv_fwd": [ctypes.POINTER(KvCacheDesc), _P, _P, _P, _P, _P, _P, _P, _P, ctypes.c_size_t, _P],
+    "pa_cache_append": [_BC, _P, _P, _I64, _I64, _I64, _I64] + [_P] * 12,
+    "pa_cache_decode_workspace_size": [_BC, _I32, _I32, ctypes.POINTER(_SIZE)],
+    "pa_cache_decode": [_BC] + [_P] * 11 + [_SIZE, _P],
+    "pa_cache_evict_workspace_size": [_BC, _I32, _I64, ctypes.POINTER(_SIZE)],
+    "pa_cache_evict": [_BC] + [_P] * 9 + [_I64, _I64, _I64] + [_P] * 5 + [_SIZE, _P],
     "pa_fwd_tile_plan": [_I32, _I32, _P],
     "pa_shard_fwd": [_I32, _P, _DESC, _P, _P, _P, _P, _P, _P],
     "pa_sdpa_bwd": [_DESC, _P, _P, _P, _P, _P, _P, _P, _P, _P, _P],
