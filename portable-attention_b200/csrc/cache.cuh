@@ -12,6 +12,25 @@ namespace pa {
 // Element kinds of a cache (template parameter of every kernel).
 enum : int { kCacheF16 = 0, kCacheBF16 = 1, kCacheE4M3 = 2, kCacheI8 = 3 };
 
+// Division of 0 <= n < 2^31 by a fixed d >= 1 as a high product, an add and a shift.
+struct FastDiv {
+  uint32_t d, mul, shift;
+};
+
+inline FastDiv make_fastdiv(uint32_t d) {
+  uint32_t s = 0;
+  while (s < 31 && (1u << s) < d) ++s;
+  const uint64_t m = ((1ull << 32) * ((1ull << s) - d)) / d + 1;
+  return {d, static_cast<uint32_t>(m), s};
+}
+
+#if defined(__CUDACC__)
+__device__ __forceinline__ int fast_div(const FastDiv& f, int n) {
+  const uint32_t u = static_cast<uint32_t>(n);
+  return static_cast<int>((__umulhi(u, f.mul) + u) >> f.shift);
+}
+#endif
+
 // What the kernels need of a checked descriptor. Strides are in bytes for the
 // cache and in elements for scales and per-row arrays.
 struct CacheView {
@@ -23,6 +42,7 @@ struct CacheView {
   int32_t kind;
   int32_t q_bf16;
   int32_t paged;
+  FastDiv by_page, by_block;
 };
 
 // Which optional parts of a descriptor a call uses.
@@ -48,7 +68,7 @@ __host__ __device__ constexpr int cache_esz(int kind) { return cache_8bit(kind) 
 __device__ __forceinline__ int32_t cache_page(const CacheView& v, const int32_t* table, int b, int row,
                                               int* status) {
   if (!table) return b;
-  const int32_t page = table[static_cast<int64_t>(b) * v.max_pages + row / v.page_size];
+  const int32_t page = table[static_cast<int64_t>(b) * v.max_pages + fast_div(v.by_page, row)];
   if (page < 0 || page >= v.num_pages) {
     atomicExch(status, kStatusBadPage);
     return -1;
@@ -56,12 +76,17 @@ __device__ __forceinline__ int32_t cache_page(const CacheView& v, const int32_t*
   return page;
 }
 
+// Place of a row inside its page.
+__device__ __forceinline__ int cache_at(const CacheView& v, int row) {
+  return v.paged ? row - fast_div(v.by_page, row) * v.page_size : row;
+}
+
 __device__ __forceinline__ int64_t cache_row(const CacheView& v, int32_t page, int h, int at) {
   return page * v.page_stride + h * v.head_stride + at * v.key_stride;
 }
 
 __device__ __forceinline__ int64_t cache_scale(const CacheView& v, int32_t page, int h, int at) {
-  return page * v.scale_page + h * v.scale_head + at / v.scale_block;
+  return page * v.scale_page + h * v.scale_head + fast_div(v.by_block, at);
 }
 
 // The least power of two s with amax <= qmax * s, at least 2^-100, by exponent

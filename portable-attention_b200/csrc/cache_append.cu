@@ -39,7 +39,7 @@ pa_status check_cache(const pa_block_cache_desc* d, const CacheUse& use, CacheVi
   }
   if (c.k_scale != 1.f || c.v_scale != 1.f)
     return fail(PA_ERR_INVALID, w + "k_scale and v_scale must be 1 (the scales are per block)");
-  if (c.max_seq_len < 0 || c.max_seq_len > kMax - 1024) return fail(PA_ERR_UNSUPPORTED, w + "too many keys");
+  if (c.max_seq_len < 0 || c.max_seq_len > kMax - 65536) return fail(PA_ERR_UNSUPPORTED, w + "too many keys");
   if (c.page_size < 1 || c.page_size > kMax) return fail(PA_ERR_INVALID, w + "page_size must be in [1, 2^31)");
   if (c.num_pages < 1 || c.num_pages > kMax) return fail(PA_ERR_INVALID, w + "num_pages must be in [1, 2^31)");
   const int esz = c.kv_dtype == PA_FP8_E4M3 || c.kv_dtype == PA_I8 ? 1 : 2;
@@ -93,6 +93,8 @@ pa_status check_cache(const pa_block_cache_desc* d, const CacheUse& use, CacheVi
   v->q_bf16 = c.q_dtype == PA_BF16;
   v->kind = c.kv_dtype == PA_FP8_E4M3 ? kCacheE4M3 : c.kv_dtype == PA_I8 ? kCacheI8 : v->q_bf16 ? kCacheBF16 : kCacheF16;
   v->paged = use.paged;
+  v->by_page = make_fastdiv(static_cast<uint32_t>(v->page_size));
+  v->by_block = make_fastdiv(static_cast<uint32_t>(v->scale_block > 0 ? v->scale_block : 1));
   return PA_OK;
 }
 
@@ -172,14 +174,14 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
       const int32_t page = cache_page(a.c, a.table, b, r, a.status);
       if (page < 0) continue;
       const uint4 w = *reinterpret_cast<const uint4*>(src + (r - len) * a.x_tok + ch * 16);
-      *reinterpret_cast<uint4*>(a.cache[kv] + cache_row(a.c, page, h, a.table ? r % a.c.page_size : r) + ch * 16) = w;
+      *reinterpret_cast<uint4*>(a.cache[kv] + cache_row(a.c, page, h, cache_at(a.c, r)) + ch * 16) = w;
     }
     return;
   }
   // 8 bits: the block lies in one page.
   const int32_t page = cache_page(a.c, a.table, b, lo, a.status);
   if (page < 0) return;
-  const int at0 = a.table ? r0 % a.c.page_size : r0;  // the block's first row inside its page
+  const int at0 = cache_at(a.c, r0);  // the block's first row inside its page
   float amax = 0.f;
   for (int i = lane; i < n; i += 32) {
     const uint4 w = *reinterpret_cast<const uint4*>(src + (lo + i / kChunks - len) * a.x_tok + (i % kChunks) * 16);

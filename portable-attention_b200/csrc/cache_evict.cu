@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const EvictAr
     // The cut block's scales, before `move` changes them.
     const int32_t page = cache_page(a.c, a.table, b, n, a.status);
     float s = 0.f;
-    if (page >= 0) s = a.scales[tid][cache_scale(a.c, page, h, a.table ? n % a.c.page_size : n)];
+    if (page >= 0) s = a.scales[tid][cache_scale(a.c, page, h, cache_at(a.c, n))];
     a.cut_scale[pair * 2 + tid] = s;
   }
   const float* w = a.weights + b * a.c.row_seq + h * a.c.row_head;
@@ -185,7 +185,7 @@ __global__ void __launch_bounds__(256) cache_move_kernel(const EvictArgs a, int3
   const int32_t* table = a.table;
   constexpr int kPieces = D * cache_esz(KIND) / 16;  // 16-byte pieces of a row
   const int total = (hi - lo) * kPieces;
-  auto place = [&](int r) { return table ? r % a.c.page_size : r; };
+  auto place = [&](int r) { return cache_at(a.c, r); };
 
   if (!cache_8bit(KIND)) {
     for (int i = lane; i < total; i += 32) {
