@@ -10,19 +10,36 @@
 // move are touched (an order-keeping compaction would move every row behind the
 // first hole).
 //
-// Two launches. `select` finds the threshold key by radix selection (four
-// passes of eight bits), the holes and their sources, and leaves in kept[] the
-// row that each place gets. `move` carries the rows, their weights and
-// positions over. In 8-bit caches a warp owns a whole scale block: it rescales
-// the block by the rule of pa_cache_append. The block that `budget` cuts holds
-// places below it and possibly sources at or above it; its old scale is put
-// aside by `select`, since `move` changes it while other warps read from it.
+// Two launches, the second started while the first ends. `select`: a (sequence,
+// kv head) is one CTA, or a cluster of up to eight where there are few of them.
+// Each thread holds eight or sixteen rows' keys in registers, four neighbours at a
+// time so that a warp's reads are whole lines (longer shares are read again in
+// rounds). The threshold key is found by radix
+// selection, digits of 11, 11 and 10 bits counted in shared memory (a cluster's
+// CTAs add their counts into each other's memory); it stops as soon as a digit's
+// rows are all taken. Ranks of ties, holes and sources are prefix sums over the
+// threads. Holes and sources go to two lists in the workspace, and the per-row
+// arrays are written. `move` carries the rows over: in 16 bits a warp takes 32
+// list entries. The call reads 8 bytes a row, writes 12 bytes a kept row and moves
+// what must move.
+//
+// In 8-bit caches a warp owns the keys or the values of a whole scale block, the
+// one whose first hole is among the eight list entries it looks at; kept[] tells
+// it what each place of the block gets, and it rescales the block by the rule of
+// pa_cache_append. The block that `budget` cuts holds places below it and
+// possibly sources at or above it: `select` puts its old scales aside, since
+// `move` changes them while other warps read from it.
 #include <math.h>
 
 #include "cache.cuh"
 
 namespace pa {
 namespace {
+
+constexpr int kBins = 2048;     // digits of 11 bits (the last: 10)
+constexpr int kScanThreads = 256;
+constexpr int kMaxThreads = 1024;
+constexpr int kMaxCluster = 8;  // portable cluster size
 
 struct EvictArgs {
   CacheView c;
@@ -36,20 +53,17 @@ struct EvictArgs {
   float* weights_out;
   int32_t* positions_out;
   int32_t* lens_out;
-  int32_t* kept;      // [B][Hkv][budget]
-  int32_t* holes;     // workspace [B][Hkv][budget]
-  float* cut_scale;   // workspace [B][Hkv][2]
+  int32_t* kept;     // [B][Hkv][budget]
+  int32_t* holes;    // workspace [B][Hkv][list]
+  int32_t* sources;  // workspace [B][Hkv][list]
+  int32_t* counts;   // workspace [B][Hkv]: moves
+  float* cut_scale;  // workspace [B][Hkv][2]: old scales of the cut block
   int* status;
-  int32_t budget, recent, sinks;
-  int32_t rows_per_block;
+  int32_t budget, recent, sinks, list;
+  int32_t cluster;   // CTAs per (sequence, kv head)
+  int32_t vec, vec_kept;  // the per-row arrays, kept[] can be used 16 bytes at a time
+  int32_t by_block;  // 8 bits: `move` has a warp for every block below the budget
 };
-
-__device__ __forceinline__ int evict_len(const EvictArgs& a, int b, bool report) {
-  const int n = a.lens[b];
-  if (n >= 0 && n <= a.c.max_len) return n;
-  if (report) atomicExch(a.status, kStatusBadSeqLen);
-  return -1;
-}
 
 // Monotonic key of a weight; -0 counts as 0, NaN as the lowest.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -58,205 +72,611 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
   return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
 
-constexpr int kSelThreads = 1024;
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile(
+      "barrier.cluster.arrive.release.aligned;\n\t"
+      "barrier.cluster.wait.acquire.aligned;" ::
+          : "memory");
+}
+__device__ __forceinline__ int cluster_load(const int* p, uint32_t rank) {
+  uint32_t at;
+  int v;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(at) : "memory");
+  return v;
+}
 
-// Inclusive ranks over the CTA of a flag; *total receives the CTA's count.
-__device__ __forceinline__ int cta_rank(bool flag, int* warp_sum, int* total) {
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const uint32_t m = __ballot_sync(0xffffffffu, flag);
+__device__ __forceinline__ void cluster_add(int* p, uint32_t rank, int v) {
+  uint32_t at;
+  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(at) : "r"(smem_u32(p)), "r"(rank));
+  asm volatile("red.relaxed.cluster.shared::cluster.add.s32 [%0], %1;" ::"r"(at), "r"(v) : "memory");
+}
+
+struct EvictShared {
+  int hist[3][kBins];  // counts of the (sequence, kv head), one array a pass
+  int own[kBins];      // clusters: this CTA's counts of the pass
+  int warp_sum[2][32];
+  int total[2];        // this CTA's ranks, read by its cluster
+  int digit, left, all;
+};
+
+// Ranks of the rows that a mask marks (bit i: row i of this thread, group i / 4
+// being 128 rows of the warp, four a lane), in row order.
+struct RowRank {
+  uint32_t before, all;  // per group, a byte each: marks of the lanes before, of the warp
+  int base;              // marks of the warps before
+  template <int kGroups>
+  __device__ __forceinline__ void count(uint32_t mask) {
+    uint32_t p = 0;
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) p |= static_cast<uint32_t>(__popc(mask >> (4 * q) & 15u)) << (8 * q);
+    uint32_t s = p;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const uint32_t y = __shfl_up_sync(0xffffffffu, s, o);
+      if (static_cast<int>(threadIdx.x & 31) >= o) s += y;
+    }
+    before = s - p;  // at most 128 in a byte: nothing carries over
+    all = __shfl_sync(0xffffffffu, s, 31);
+  }
+  __device__ __forceinline__ int warp_total() const {
+    return (all & 255u) + (all >> 8 & 255u) + (all >> 16 & 255u) + (all >> 24);
+  }
+  // Rank of the first row of group q.
+  __device__ __forceinline__ int group(int q) const {
+    int r = base + (before >> (8 * q) & 255u);
+    for (int i = 0; i < q; ++i) r += all >> (8 * i) & 255u;
+    return r;
+  }
+};
+
+// Exclusive prefix sum over the CTA's threads; `total` receives the sum.
+__device__ __forceinline__ int cta_scan(int x, int* warp_sum, int* total) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  int s = x;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, s, o);
+    if (lane >= o) s += y;
+  }
   __syncthreads();  // earlier readers of warp_sum are done
-  if (lane == 0) warp_sum[warp] = __popc(m);
+  if (lane == 31) warp_sum[warp] = s;
   __syncthreads();
-  int before = 0, all = 0;
-  for (int w = 0; w < kSelThreads / 32; ++w) {
-    const int n = warp_sum[w];
-    before += w < warp ? n : 0;
-    all += n;
+  int w = lane < warps ? warp_sum[lane] : 0;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int y = __shfl_up_sync(0xffffffffu, w, o);
+    if (lane >= o) w += y;
   }
-  *total = all;
-  return before + __popc(m & ((2u << lane) - 1u));
+  *total = __shfl_sync(0xffffffffu, w, 31);
+  const int before = __shfl_sync(0xffffffffu, w, warp > 0 ? warp - 1 : 0);
+  return (warp > 0 ? before : 0) + s - x;
 }
 
-__global__ void __launch_bounds__(kSelThreads) cache_select_kernel(const EvictArgs a) {
-  __shared__ int hist[256];
-  __shared__ int warp_sum[kSelThreads / 32];
-  __shared__ uint32_t s_prefix;
-  __shared__ int s_left;
-  const int h = blockIdx.x % a.c.Hkv, b = blockIdx.x / a.c.Hkv;
-  const int tid = threadIdx.x;
-  const int len = evict_len(a, b, tid == 0 && h == 0);
-  const int n = a.budget;
-  const int64_t pair = blockIdx.x;
-  int32_t* kept = a.kept + pair * n;
-  int32_t* holes = a.holes + pair * n;
-  if (h == 0 && tid == 0) a.lens_out[b] = len < 0 ? a.lens[b] : (len < n ? len : n);
-  if (len <= n) {
-    for (int r = tid; r < n; r += kSelThreads) kept[r] = r < len ? r : -1;
-    return;
+// Sums of x and y over the warps before this one, and over all of them.
+__device__ __forceinline__ int4 warps_before(int x, int y, int (*warp_sum)[32]) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, warps = blockDim.x >> 5;
+  __syncthreads();  // earlier readers of warp_sum are done
+  if (lane == 0) {
+    warp_sum[0][warp] = x;
+    warp_sum[1][warp] = y;
   }
-  if (cache_8bit(a.c.kind) && tid < 2 && n % a.rows_per_block) {
-    // The cut block's scales, before `move` changes them.
-    const int32_t page = cache_page(a.c, a.table, b, n, a.status);
-    float s = 0.f;
-    if (page >= 0) s = a.scales[tid][cache_scale(a.c, page, h, cache_at(a.c, n))];
-    a.cut_scale[pair * 2 + tid] = s;
-  }
-  const float* w = a.weights + b * a.c.row_seq + h * a.c.row_head;
-  const int32_t* pos = a.positions ? a.positions + b * a.c.row_seq + h * a.c.row_head : nullptr;
-  const int64_t next = a.next ? a.next[b] : len;
-  auto key_of = [&](int r) -> uint32_t {
-    const int p = pos ? pos[r] : r;
-    if (p >= next - a.recent || p < a.sinks) return 0xffffffffu;
-    return weight_key(w[r]);
-  };
-  uint32_t prefix = 0;
-  int left = n;  // rows still to take among those that match the prefix
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelThreads) hist[i] = 0;
-    __syncthreads();
-    for (int r = tid; r < len; r += kSelThreads) {
-      const uint32_t key = key_of(r);
-      if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255u], 1);
-    }
-    __syncthreads();
-    if (tid == 0) {
-      int d = 255, t = left;
-      while (d > 0 && hist[d] < t) t -= hist[d--];
-      s_prefix = prefix | (static_cast<uint32_t>(d) << shift);
-      s_left = t;
-    }
-    __syncthreads();
-    prefix = s_prefix;
-    left = s_left;
-  }
-  // Rows above the key `prefix` are kept, and the first `left` rows that equal it.
-  int ties = 0, n_holes = 0, n_src = 0;
-  for (int base = 0; base < len; base += kSelThreads) {
-    const int r = base + tid;
-    const uint32_t key = r < len ? key_of(r) : 0u;
-    const bool tie = r < len && key == prefix;
-    int total;
-    const int tie_rank = ties + cta_rank(tie, warp_sum, &total);
-    ties += total;
-    const bool keep = r < len && (key > prefix || (tie && tie_rank <= left));
-    if (base < n) {
-      const bool hole = r < n && !keep;
-      const int rank = n_holes + cta_rank(hole, warp_sum, &total);
-      n_holes += total;
-      if (hole) holes[rank - 1] = r;
-      if (r < n && keep) kept[r] = r;
-      __syncthreads();  // the holes are in memory before a source looks one up
-    }
-    const bool src = r >= n && keep;
-    const int rank = n_src + cta_rank(src, warp_sum, &total);
-    n_src += total;
-    if (src) kept[holes[rank - 1]] = r;
-  }
+  __syncthreads();
+  const int u = lane < warps ? warp_sum[0][lane] : 0, v = lane < warps ? warp_sum[1][lane] : 0;
+  return make_int4(__reduce_add_sync(0xffffffffu, lane < warp ? u : 0), __reduce_add_sync(0xffffffffu, lane < warp ? v : 0),
+                   __reduce_add_sync(0xffffffffu, u), __reduce_add_sync(0xffffffffu, v));
 }
 
-// A warp moves the rows of one block of places of one (sequence, kv head).
+// Codes of a 16-byte piece under another scale, stored at p. A power of two
+// divides exactly as a product with its reciprocal.
+template <int KIND, bool POW2>
+__device__ __forceinline__ void recode(const uint4& q, float s, float to, float inv, uint8_t* p) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t o[4] = {0u, 0u, 0u, 0u};
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float2 f = cache_dec2<KIND>(w[e >> 1] >> (16 * (e & 1)));
+    const float y = f.x * s, z = f.y * s;
+    o[e >> 1] |= (POW2 ? cache_enc2<KIND>(y * inv, z * inv) : cache_enc2<KIND>(__fdiv_rn(y, to), __fdiv_rn(z, to)))
+                 << (16 * (e & 1));
+  }
+  *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+}
+
+// Moves into the scale block of rows lo.. of a cache's keys or values, by one
+// warp: places are taken 16 or 32 at a time, lane i looking up place i's source,
+// then rows are read in four rounds. One step stays in registers between the
+// maximum and the coding; larger blocks are read again.
 template <int KIND, int D>
-__global__ void __launch_bounds__(256) cache_move_kernel(const EvictArgs a, int32_t blocks, int64_t items) {
+__device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo) {
+  constexpr int kPieces = D / 16;      // lanes per row
+  constexpr int kRows = 32 / kPieces;  // rows per round of a warp
+  constexpr int kStep = 4 * kRows;     // places per step: 16 or 32
   const int lane = threadIdx.x & 31;
-  const int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
-  if (item >= items) return;
-  const int h = static_cast<int>(item % a.c.Hkv);
-  const int64_t rest = item / a.c.Hkv;
-  const int blk = static_cast<int>(rest % blocks);
-  const int b = static_cast<int>(rest / blocks);
-  const int len = evict_len(a, b, false);
-  const int n = a.budget, bs = a.rows_per_block;
-  const int64_t pair = static_cast<int64_t>(b) * a.c.Hkv + h;
+  const int bs = a.c.scale_block, n = a.budget;
+  const int hi = lo + bs < n ? lo + bs : n;
+  const int cut = n % bs ? n / bs : -1;  // the block whose old scales were put aside
+  const int ch = (lane % kPieces) * 16;
   const int32_t* kept = a.kept + pair * n;
-  const int lo = blk * bs;
-  int hi = lo + bs < n ? lo + bs : n;
-  hi = hi < len ? hi : len;
-  if (lo >= hi) return;
-  const int64_t row0 = b * a.c.row_seq + h * a.c.row_head;
-  int moved = 0;
-  for (int r = lo + lane; r < hi; r += 32) {
-    const int src = kept[r];
-    moved += src != r;
-    if (a.weights_out) a.weights_out[row0 + r] = a.weights[row0 + src];
-    if (a.positions_out) a.positions_out[row0 + r] = a.positions ? a.positions[row0 + src] : src;
-  }
-  moved = __reduce_add_sync(0xffffffffu, moved);
-  if (moved == 0) return;
-  const int32_t* table = a.table;
-  constexpr int kPieces = D * cache_esz(KIND) / 16;  // 16-byte pieces of a row
-  const int total = (hi - lo) * kPieces;
-  auto place = [&](int r) { return cache_at(a.c, r); };
-
-  if (!cache_8bit(KIND)) {
-    for (int i = lane; i < total; i += 32) {
-      const int r = lo + i / kPieces, ch = i % kPieces;
+  uint8_t* cache = kv ? a.cache[1] : a.cache[0];
+  float* scales = kv ? a.scales[1] : a.scales[0];
+  const int32_t page = cache_page(a.c, a.table, b, lo, a.status);
+  if (page < 0) return;
+  const int at_lo = cache_at(a.c, lo);
+  float* const sp = scales + cache_scale(a.c, page, h, at_lo);
+  uint8_t* const dst0 = cache + cache_row(a.c, page, h, at_lo) + ch;
+  const float was = *sp;
+  int64_t from = -1;   // place `lane`: its source row (-1: it stays, or a bad page)
+  float scale = 0.f;   // and the source's scale
+  bool stays = false;  // some place keeps its row
+  auto look_up = [&](int first) {
+    from = -1;
+    scale = 0.f;
+    const int r = first + lane;
+    if (lane < kStep && r < hi) {
       const int src = kept[r];
-      if (src == r) continue;
-      const int32_t pd = cache_page(a.c, table, b, r, a.status), ps = cache_page(a.c, table, b, src, a.status);
-      if (pd < 0 || ps < 0) continue;
-      const int64_t d = cache_row(a.c, pd, h, place(r)) + ch * 16, s = cache_row(a.c, ps, h, place(src)) + ch * 16;
+      if (src == r) {
+        stays = true;
+      } else {
+        const int32_t ps = cache_page(a.c, a.table, b, src, a.status);
+        if (ps >= 0) {
+          const int at = cache_at(a.c, src);
+          from = cache_row(a.c, ps, h, at);
+          scale = src / bs == cut ? a.cut_scale[pair * 2 + kv] : scales[cache_scale(a.c, ps, h, at)];
+        }
+      }
+    }
+  };
+  uint4 x[4];
+  auto read = [&]() {
 #pragma unroll
-      for (int kv = 0; kv < 2; ++kv)
-        *reinterpret_cast<uint4*>(a.cache[kv] + d) = *reinterpret_cast<const uint4*>(a.cache[kv] + s);
+    for (int u = 0; u < 4; ++u) {
+      const int64_t f = __shfl_sync(0xffffffffu, from, u * kRows + lane / kPieces);
+      x[u] = f >= 0 ? *reinterpret_cast<const uint4*>(cache + f + ch) : make_uint4(0u, 0u, 0u, 0u);
+    }
+  };
+  float amax = 0.f;
+  for (int first = lo; first < hi; first += kStep) {
+    look_up(first);
+    read();
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const float s = __shfl_sync(0xffffffffu, scale, u * kRows + lane / kPieces);
+      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+      float m = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float2 f = cache_dec2<KIND>(w[e >> 1] >> (16 * (e & 1)));
+        m = cache_amax(cache_amax(m, f.x), f.y);
+      }
+      amax = cache_amax(amax, m * s);
+    }
+  }
+  const bool held = __any_sync(0xffffffffu, stays);
+  const float need = cache_need_scale<KIND>(warp_max(amax));
+  const float old = held ? was : 0.f;
+  const float to = old > need ? old : need;
+  const bool pow2 = (__float_as_uint(to) & 0x807fffffu) == 0u;
+  const float inv = __fdiv_rn(1.f, to);
+  for (int first = lo; first < hi; first += kStep) {
+    if (hi - lo > kStep) {
+      look_up(first);
+      read();
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = u * kRows + lane / kPieces;
+      const int64_t f = __shfl_sync(0xffffffffu, from, j);
+      const float s = __shfl_sync(0xffffffffu, scale, j);
+      if (f < 0) continue;
+      uint8_t* p = dst0 + (first + j - lo) * a.c.key_stride;
+      if (pow2)
+        recode<KIND, true>(x[u], s, to, inv, p);
+      else
+        recode<KIND, false>(x[u], s, to, inv, p);
+    }
+  }
+  if (held && to != old) {
+    for (int r = lo + lane / kPieces; r < hi; r += kRows) {
+      if (kept[r] != r) continue;
+      uint8_t* p = dst0 + (r - lo) * a.c.key_stride;
+      recode<KIND, false>(*reinterpret_cast<const uint4*>(p), old, to, inv, p);
+    }
+  }
+  __syncwarp();
+  if (lane == 0) *sp = to;
+}
+
+// kThreads and kCtas bound the registers: 1024 threads, or four CTAs of up to 320
+// for many short sequences, so that 512 of them run at once.
+template <int kKeys, int kThreads, int kCtas>
+__global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const EvictArgs a) {
+  extern __shared__ __align__(16) uint8_t smem_raw[];
+  EvictShared& sh = *reinterpret_cast<EvictShared*>(smem_raw);
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int C = a.cluster;
+  const int rank = blockIdx.x % C;
+  const int64_t pair = blockIdx.x / C;
+  const int h = static_cast<int>(pair % a.c.Hkv), b = static_cast<int>(pair / a.c.Hkv);
+  const int tid = threadIdx.x, T = blockDim.x;
+  const int n = a.budget;
+  int len = a.lens[b];
+  const int32_t* pos = a.positions ? a.positions + b * a.c.row_seq + h * a.c.row_head : nullptr;
+  const float* w = a.weights + b * a.c.row_seq + h * a.c.row_head;
+  float* w_out = a.weights_out ? a.weights_out + b * a.c.row_seq + h * a.c.row_head : nullptr;
+  int32_t* p_out = a.positions_out ? a.positions_out + b * a.c.row_seq + h * a.c.row_head : nullptr;
+  int32_t* kept = a.kept + pair * n;
+  int32_t* holes = a.holes + pair * a.list;
+  int32_t* sources = a.sources + pair * a.list;
+  const bool bad = len < 0 || len > a.c.max_len;
+  if (h == 0 && rank == 0 && tid == 0) {
+    if (bad) atomicExch(a.status, kStatusBadSeqLen);
+    a.lens_out[b] = bad ? len : (len < n ? len : n);
+  }
+  if (bad) len = 0;
+  if (len <= n) {  // nothing to evict (the whole cluster leaves here)
+    if (rank == 0 && tid == 0) a.counts[pair] = 0;
+    for (int64_t r = rank * T + tid; r < n; r += C * T) {
+      kept[r] = r < len ? static_cast<int32_t>(r) : -1;
+      if (r < len && w_out) w_out[r] = w[r];
+      if (r < len && p_out) p_out[r] = pos ? pos[r] : static_cast<int32_t>(r);
     }
     return;
   }
-  const int32_t page = cache_page(a.c, table, b, lo, a.status);
-  if (page < 0) return;
-  const int cut = n % bs ? n / bs : -1;  // the block whose old scales were put aside
+  auto sync_all = [&]() {
+    if (C > 1)
+      cluster_sync();
+    else
+      __syncthreads();
+  };
+  // This CTA's rows: [row0, row_end), in rounds of T * kKeys.
+  const int share = ((len + C - 1) / C + 3) / 4 * 4;
+  const int64_t row0 = static_cast<int64_t>(rank) * share;
+  const int64_t row_end = row0 + share < len ? row0 + share : len;
+  const int per_round = T * kKeys;
+  const int rounds = (share + per_round - 1) / per_round;
+  const int64_t next = a.next ? a.next[b] : len;
+  const int64_t newest = next - a.recent;
+  constexpr int kGroups = kKeys / 4;
+  const int lane = tid & 31;
+  uint32_t keys[kKeys];
+  uint32_t live = 0;   // rows this thread holds in the current round
+  int64_t my_row = 0;  // the first of them; group q starts 128 q further on
+  auto row_of = [&](int i) { return my_row + (i / 4) * 128 + (i & 3); };
+  auto load_keys = [&](int round) {
+    my_row = row0 + static_cast<int64_t>(round) * per_round + (tid >> 5) * (32 * kKeys) + lane * 4;
+    live = 0;
+    float4 wv[kGroups];
+    int4 pv[kGroups];
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      const int64_t r = my_row + q * 128;
+      wv[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      pv[q] = make_int4(0, 0, 0, 0);
+      if (r + 4 <= row_end && a.vec) {
+        wv[q] = *reinterpret_cast<const float4*>(w + r);
+        if (pos) pv[q] = *reinterpret_cast<const int4*>(pos + r);
+        live |= 15u << (4 * q);
+      } else if (r < row_end) {
+        float* wf = &wv[q].x;
+        int* pf = &pv[q].x;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (r + e < row_end) {
+            wf[e] = w[r + e];
+            if (pos) pf[e] = pos[r + e];
+            live |= 1u << (4 * q + e);
+          }
+      }
+    }
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      const float wf[4] = {wv[q].x, wv[q].y, wv[q].z, wv[q].w};
+      const int pf[4] = {pv[q].x, pv[q].y, pv[q].z, pv[q].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int64_t p = pos ? pf[e] : my_row + q * 128 + e;
+        keys[4 * q + e] = p >= newest || p < a.sinks ? 0xffffffffu : weight_key(wf[e]);
+      }
+    }
+  };
+
+  // ------------------------------------------------ threshold: radix selection
+  for (int i = tid; i < 4 * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
+  load_keys(0);
+  sync_all();
+  uint32_t prefix = 0;
+  int left = n;  // rows to take among those that match the prefix
+  bool all = false;
 #pragma unroll 1
-  for (int kv = 0; kv < 2; ++kv) {
-    auto src_scale = [&](int32_t ps, int src) -> float {
-      if (src / bs == cut) return a.cut_scale[pair * 2 + kv];
-      return a.scales[kv][cache_scale(a.c, ps, h, place(src))];
-    };
-    float amax = 0.f;
-    for (int i = lane; i < total; i += 32) {
-      const int r = lo + i / kPieces, ch = i % kPieces;
-      const int src = kept[r];
-      if (src == r) continue;
-      const int32_t ps = cache_page(a.c, table, b, src, a.status);
-      if (ps < 0) continue;
-      const float s = src_scale(ps, src);
-      const uint4 w = *reinterpret_cast<const uint4*>(a.cache[kv] + cache_row(a.c, ps, h, place(src)) + ch * 16);
-      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
+  for (int pass = 0; pass < 3; ++pass) {
+    const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0;
+    const int width = pass == 2 ? 10 : 11;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load_keys(round);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float2 f = cache_dec2<KIND>(wd[k >> 1] >> (16 * (k & 1)));
-        amax = cache_amax(cache_amax(amax, f.x * s), f.y * s);
+      for (int i = 0; i < kKeys; ++i)
+        if ((live >> i & 1u) && (pass == 0 || (keys[i] >> (shift + width)) == (prefix >> (shift + width))))
+          atomicAdd((C > 1 ? sh.own : sh.hist[pass]) + ((keys[i] >> shift) & ((1u << width) - 1u)), 1);
+    }
+    if (C > 1) {
+      __syncthreads();
+      for (int i = tid; i < kBins; i += T) {
+        const int x = sh.own[i];
+        if (x == 0) continue;
+        sh.own[i] = 0;
+        for (int q = 0; q < C; ++q) cluster_add(&sh.hist[pass][i], q, x);
       }
     }
-    amax = warp_max(amax);
-    float* sp = a.scales[kv] + cache_scale(a.c, page, h, place(lo));
-    const bool held = moved < hi - lo;
-    const float need = cache_need_scale<KIND>(amax);
-    const float old = held ? *sp : 0.f;
-    const float s_new = old > need ? old : need;
-    for (int i = lane; i < total; i += 32) {
-      const int r = lo + i / kPieces, ch = i % kPieces;
-      const int src = kept[r];
-      if (src == r && s_new == old) continue;
-      const int32_t ps = src == r ? page : cache_page(a.c, table, b, src, a.status);
-      if (ps < 0) continue;
-      const float s = src == r ? old : src_scale(ps, src);
-      const uint4 w = *reinterpret_cast<const uint4*>(a.cache[kv] + cache_row(a.c, ps, h, place(src)) + ch * 16);
-      const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-      uint32_t o[4] = {0u, 0u, 0u, 0u};
+    sync_all();
+    // Thread t < 256 takes bins 8 t' .. 8 t' + 7 from the top, t' = 255 - t.
+    int bins[kBins / kScanThreads], sum = 0;
+    if (tid < kScanThreads) {
+      const int first = (kScanThreads - 1 - tid) * (kBins / kScanThreads);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float2 f = cache_dec2<KIND>(wd[k >> 1] >> (16 * (k & 1)));
-        o[k >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x * s, s_new), __fdiv_rn(f.y * s, s_new)) << (16 * (k & 1));
+      for (int i = 0; i < kBins / kScanThreads; ++i) {
+        bins[i] = sh.hist[pass][first + i];
+        sum += bins[i];
       }
-      *reinterpret_cast<uint4*>(a.cache[kv] + cache_row(a.c, page, h, place(r)) + ch * 16) =
-          make_uint4(o[0], o[1], o[2], o[3]);
     }
-    __syncwarp();  // every lane has read the old scale
-    if (lane == 0) *sp = s_new;
+    int total;
+    int above = cta_scan(sum, sh.warp_sum[0], &total);
+    if (tid < kScanThreads && above < left && above + sum >= left) {
+      const int first = (kScanThreads - 1 - tid) * (kBins / kScanThreads);
+#pragma unroll
+      for (int i = kBins / kScanThreads - 1; i >= 0; --i) {
+        if (above < left && above + bins[i] >= left) {
+          sh.digit = first + i;
+          sh.left = left - above;
+          sh.all = bins[i] == left - above;
+        }
+        above += bins[i];
+      }
+    }
+    __syncthreads();
+    prefix |= static_cast<uint32_t>(sh.digit) << shift;
+    left = sh.left;
+    all = sh.all != 0;
+    if (all) break;  // every row with this prefix is taken: no need to look further
+  }
+
+  // --------------------------------------------- ranks of ties, holes, sources
+  // Kept: keys above the prefix, and of the keys that equal it the first `left`
+  // (all keys from the prefix up, where `all`). Two sweeps: the counts of each
+  // CTA, then, with the counts of the CTAs before it, the lists.
+  // Sums of total[0] and total[1] over the CTAs before this one, and of total[0] over all.
+  auto before = [&](const int* total) -> int4 {
+    const int x = lane < C ? cluster_load(total, lane) : 0, y = lane < C ? cluster_load(total + 1, lane) : 0;
+    return make_int4(__reduce_add_sync(0xffffffffu, lane < rank ? x : 0),
+                     __reduce_add_sync(0xffffffffu, lane < rank ? y : 0), __reduce_add_sync(0xffffffffu, x), 0);
+  };
+  int tie_base = 0;
+  if (!all) {
+    int own = 0;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load_keys(round);
+#pragma unroll
+      for (int i = 0; i < kKeys; ++i) own += (live >> i & 1u) && keys[i] == prefix;
+    }
+    if (C > 1) {
+      int total;
+      cta_scan(own, sh.warp_sum[0], &total);
+      if (tid == 0) sh.total[0] = total;
+      cluster_sync();
+      tie_base = before(sh.total).x;
+      cluster_sync();  // total is used again
+    }
+  }
+  int hole_base = 0, src_base = 0, hole_all = 0;
+  uint32_t keep = 0, hole = 0, src = 0;
+  RowRank holes_at, src_at;
+  int round_holes = 0, round_src = 0;
+  // The current round's masks, and ranks inside it.
+  auto rank_round = [&](int& ties) {
+    keep = 0;
+    uint32_t tie = 0;
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) {
+      if (all ? keys[i] >= prefix : keys[i] > prefix) keep |= 1u << i;
+      if (!all && keys[i] == prefix) tie |= 1u << i;
+    }
+    keep &= live;
+    tie &= live;
+    if (!all) {
+      RowRank at;
+      at.count<kGroups>(tie);
+      const int4 sum = warps_before(at.warp_total(), 0, sh.warp_sum);
+      at.base = ties + sum.x;
+      ties += sum.z;
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        int r = at.group(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (tie >> (4 * q + e) & 1u) {
+            if (r < left) keep |= 1u << (4 * q + e);
+            ++r;
+          }
+      }
+    }
+    uint32_t low = 0;  // rows below the budget
+#pragma unroll
+    for (int i = 0; i < kKeys; ++i) low |= row_of(i) < n ? 1u << i : 0u;
+    hole = ~keep & live & low;
+    src = keep & ~low;
+    holes_at.count<kGroups>(hole);
+    src_at.count<kGroups>(src);
+    const int4 sum = warps_before(holes_at.warp_total(), src_at.warp_total(), sh.warp_sum);
+    holes_at.base = sum.x;
+    src_at.base = sum.y;
+    round_holes = sum.z;
+    round_src = sum.w;
+  };
+  if (C > 1) {
+    int ties = tie_base, n_hole = 0, n_src = 0;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load_keys(round);
+      rank_round(ties);
+      n_hole += round_holes;
+      n_src += round_src;
+    }
+    if (tid == 0) {
+      sh.total[0] = n_hole;
+      sh.total[1] = n_src;
+    }
+    cluster_sync();
+    const int4 x = before(sh.total);
+    hole_base = x.x;
+    src_base = x.y;
+    hole_all = x.z;
+  }
+  const bool copy_w = w_out && w_out != w, copy_p = p_out && p_out != pos;
+  {
+    int ties = tie_base, n_hole = hole_base, n_src = src_base;
+#pragma unroll 1
+    for (int round = 0; round < rounds; ++round) {
+      if (rounds > 1) load_keys(round);
+      if (rounds > 1 || C == 1) rank_round(ties);  // else the ranks are still there
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        int hr = n_hole + holes_at.group(q), sr = n_src + src_at.group(q);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int i = 4 * q + e;
+          if (hole >> i & 1u) holes[hr++] = static_cast<int32_t>(row_of(i));
+          if (src >> i & 1u) sources[sr++] = static_cast<int32_t>(row_of(i));
+        }
+      }
+      // Rows that stay.
+#pragma unroll
+      for (int q = 0; q < kGroups; ++q) {
+        const uint32_t stay = keep & ~src;
+        const int64_t r = my_row + q * 128;
+        if ((stay >> (4 * q) & 15u) == 15u && a.vec) {
+          const int32_t r32 = static_cast<int32_t>(r);
+          if (copy_w) *reinterpret_cast<float4*>(w_out + r) = *reinterpret_cast<const float4*>(w + r);
+          if (copy_p)
+            *reinterpret_cast<int4*>(p_out + r) =
+                pos ? *reinterpret_cast<const int4*>(pos + r) : make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
+          if (a.vec_kept)
+            *reinterpret_cast<int4*>(kept + r) = make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
+          else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) kept[r + e] = r32 + e;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (stay >> (4 * q + e) & 1u) {
+              kept[r + e] = static_cast<int32_t>(r + e);
+              if (copy_w) w_out[r + e] = w[r + e];
+              if (copy_p) p_out[r + e] = pos ? pos[r + e] : static_cast<int32_t>(r + e);
+            }
+        }
+      }
+      n_hole += round_holes;
+      n_src += round_src;
+      if (C == 1) hole_all = n_hole;
+    }
+  }
+  sync_all();  // the lists are complete
+  for (int k = rank * T + tid; k < hole_all; k += C * T) {
+    const int d = holes[k], q = sources[k];
+    kept[d] = q;
+    if (w_out) w_out[d] = w[q];
+    if (p_out) p_out[d] = pos ? pos[q] : q;
+  }
+  if (rank == 0 && tid == 0) a.counts[pair] = hole_all;
+  if (cache_8bit(a.c.kind) && rank == 0 && tid < 2 && n % a.c.scale_block) {
+    const int32_t page = cache_page(a.c, a.table, b, n, a.status);
+    a.cut_scale[pair * 2 + tid] = page < 0 ? 0.f : a.scales[tid][cache_scale(a.c, page, h, cache_at(a.c, n))];
+  }
+}
+
+// 16 bits: a warp moves the rows of 32 list entries. 8 bits: where moves can be as
+// many as blocks, a warp has one block's keys or values; where they are fewer, it
+// looks at eight entries and moves the scale blocks whose first hole is among
+// them. The chain of look-ups is what takes the time, hence the many warps.
+constexpr int move_entries(int kind) { return cache_8bit(kind) ? 8 : 32; }
+
+template <int KIND, int D>
+__global__ void __launch_bounds__(256, 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
+  int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
+  if (item >= items) return;
+  const int lane = threadIdx.x & 31;
+  const int kv = cache_8bit(KIND) ? static_cast<int>(item & 1) : 0;
+  if (cache_8bit(KIND)) item >>= 1;
+  const int64_t pair = item / chunks;
+  const int chunk = static_cast<int>(item % chunks);
+  const int h = static_cast<int>(pair % a.c.Hkv), b = static_cast<int>(pair / a.c.Hkv);
+  const int32_t* holes = a.holes + pair * a.list;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  const int m = a.counts[pair];
+  if (cache_8bit(KIND) && a.by_block) {
+    const int lo = chunk * a.c.scale_block;
+    const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
+    bool moved = false;
+    if (m > 0)
+      for (int r = lo + lane; r < hi; r += 32) moved = moved || a.kept[pair * a.budget + r] != r;
+    if (__any_sync(0xffffffffu, moved)) move_block<KIND, D>(a, kv, b, h, pair, lo);
+    return;
+  }
+  const int k0 = chunk * move_entries(KIND);
+  if (k0 >= m) return;
+  const int k = k0 + lane;
+  const int cnt = m - k0 < move_entries(KIND) ? m - k0 : move_entries(KIND);
+  if (cache_8bit(KIND)) {
+    const int bs = a.c.scale_block;
+    const int block = lane < cnt ? holes[k] / bs : -1;
+    const int prev = lane < cnt && k > 0 ? holes[k - 1] / bs : -1;
+    uint32_t leads = __ballot_sync(0xffffffffu, lane < cnt && block != prev);
+    while (leads) {
+      const int l = __ffs(leads) - 1;
+      leads &= leads - 1;
+      move_block<KIND, D>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs);
+    }
+  } else {
+    constexpr int kPieces = D / 8;       // lanes per row
+    constexpr int kRows = 32 / kPieces;  // rows per step of a warp
+    int64_t from = -1, to = -1;
+    if (lane < cnt) {
+      const int dst = holes[k], src = a.sources[pair * a.list + k];
+      const int32_t pd = cache_page(a.c, a.table, b, dst, a.status), ps = cache_page(a.c, a.table, b, src, a.status);
+      if (pd >= 0 && ps >= 0) {
+        to = cache_row(a.c, pd, h, cache_at(a.c, dst));
+        from = cache_row(a.c, ps, h, cache_at(a.c, src));
+      }
+    }
+    const int ch = (lane % kPieces) * 16;
+    for (int i = 0; i < cnt; i += 4 * kRows) {
+      uint4 x[4][2];
+      int64_t d[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const int j = i + u * kRows + lane / kPieces;
+        const int64_t s = __shfl_sync(0xffffffffu, from, j & 31);
+        d[u] = __shfl_sync(0xffffffffu, to, j & 31);
+        if (j >= cnt) d[u] = -1;
+        if (d[u] >= 0) {
+          x[u][0] = *reinterpret_cast<const uint4*>(a.cache[0] + s + ch);
+          x[u][1] = *reinterpret_cast<const uint4*>(a.cache[1] + s + ch);
+        }
+      }
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+        if (d[u] >= 0) {
+          *reinterpret_cast<uint4*>(a.cache[0] + d[u] + ch) = x[u][0];
+          *reinterpret_cast<uint4*>(a.cache[1] + d[u] + ch) = x[u][1];
+        }
+    }
   }
 }
 
 struct EvictPlan {
   CacheView c;
+  int64_t list;  // most moves of a (sequence, kv head)
   size_t bytes;
 };
 
@@ -265,22 +685,57 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
   PA_TRY(check_cache(d, {paged, true, false}, &p->c, "cache evict"));
   if (budget < 1 || budget > 0x7fffffffLL - 1024) return fail(PA_ERR_INVALID, "cache evict: budget must be in [1, 2^31)");
   const size_t pairs = static_cast<size_t>(p->c.B) * p->c.Hkv;
-  p->bytes = pairs * (2 * sizeof(float) + static_cast<size_t>(budget) * sizeof(int32_t));
-  if (pairs > 0x7fffffffu) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
+  const int64_t over = p->c.max_len > budget ? p->c.max_len - budget : 0;
+  p->list = over < budget ? over : budget;
+  p->bytes = pairs * (3 + 2 * static_cast<size_t>(p->list)) * sizeof(int32_t);
+  if (pairs * kMaxCluster > 0x7fffffffu) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
   return PA_OK;
 }
 
+// A CTA per (sequence, kv head), or a cluster of 2, 4 or 8 while that leaves SMs
+// without work and every CTA 2048 rows; threads for eight rows each, sixteen
+// where 1024 threads of eight would need a second round.
 template <int KIND, int D>
-pa_status launch_evict(const EvictArgs& a, cudaStream_t st) {
-  cache_select_kernel<<<static_cast<unsigned>(a.c.B) * a.c.Hkv, kSelThreads, 0, st>>>(a);
-  PA_CUDA(cudaGetLastError());
-  const int32_t top = a.budget < a.c.max_len ? a.budget : a.c.max_len;
-  const int32_t blocks = static_cast<int32_t>((static_cast<int64_t>(top) + a.rows_per_block - 1) / a.rows_per_block);
-  const int64_t items = static_cast<int64_t>(a.c.B) * a.c.Hkv * blocks;
-  if (items == 0) return PA_OK;
+pa_status launch_evict(EvictArgs a, cudaStream_t st) {
+  const int64_t pairs = static_cast<int64_t>(a.c.B) * a.c.Hkv;
+  int cluster = 1;
+  while (cluster < kMaxCluster && pairs * cluster * 2 <= 2 * sm_count() && a.c.max_len / (2 * cluster) >= 2048) cluster *= 2;
+  a.cluster = cluster;
+  const int64_t share = (static_cast<int64_t>(a.c.max_len) + cluster - 1) / cluster;
+  const int keys = share > 8 * kMaxThreads ? 16 : 8;
+  int64_t threads = ((share + keys - 1) / keys + 31) / 32 * 32;
+  threads = threads < kScanThreads ? kScanThreads : threads > kMaxThreads ? kMaxThreads : threads;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = static_cast<unsigned>(cluster);
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(static_cast<unsigned>(pairs * cluster));
+  cfg.blockDim = dim3(static_cast<unsigned>(threads));
+  cfg.dynamicSmemBytes = sizeof(EvictShared);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = cluster > 1 ? 1 : 0;
+  PA_CUDA(cudaLaunchKernelEx(&cfg, keys == 16       ? cache_select_kernel<16, kMaxThreads, 1>
+                                   : threads <= 320 ? cache_select_kernel<8, 320, 4>
+                                                    : cache_select_kernel<8, kMaxThreads, 1>, a));
+  if (a.list == 0) return PA_OK;
+  int32_t chunks = (a.list + move_entries(KIND) - 1) / move_entries(KIND);
+  if (cache_8bit(KIND)) {
+    const int32_t blocks = (a.budget + a.c.scale_block - 1) / a.c.scale_block;
+    a.by_block = a.list >= blocks;
+    if (a.by_block) chunks = blocks;
+  }
+  const int64_t items = pairs * chunks * (cache_8bit(KIND) ? 2 : 1);
   if ((items + 7) / 8 > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
-  cache_move_kernel<KIND, D><<<static_cast<unsigned>((items + 7) / 8), 256, 0, st>>>(a, blocks, items);
-  PA_CUDA(cudaGetLastError());
+  // Starts while `select` ends; waits for its memory.
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.numAttrs = 1;
+  cfg.gridDim = dim3(static_cast<unsigned>((items + 7) / 8));
+  cfg.blockDim = dim3(256);
+  cfg.dynamicSmemBytes = 0;
+  PA_CUDA(cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D>, a, chunks, items));
   return PA_OK;
 }
 
@@ -353,12 +808,18 @@ extern "C" pa_status pa_cache_evict(const pa_block_cache_desc* desc, void* k_cac
   a.budget = static_cast<int32_t>(budget);
   a.recent = static_cast<int32_t>(recent);
   a.sinks = static_cast<int32_t>(sinks);
-  // 16-bit caches have no blocks: 16 rows make an item.
-  a.rows_per_block = cache_8bit(p.c.kind) ? p.c.scale_block : 16;
+  a.list = static_cast<int32_t>(p.list);
+  a.vec = ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(positions) |
+            reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(positions_out)) & 15) == 0 &&
+          p.c.row_head % 4 == 0 && p.c.row_seq % 4 == 0;
+  a.vec_kept = (reinterpret_cast<uintptr_t>(kept) & 15) == 0 && budget % 4 == 0;
   void* own = nullptr;
   if (!workspace) PA_TRY(scratch_alloc(&own, p.bytes, st));
+  const size_t pairs = static_cast<size_t>(p.c.B) * p.c.Hkv;
   a.cut_scale = static_cast<float*>(workspace ? workspace : own);
-  a.holes = reinterpret_cast<int32_t*>(a.cut_scale + static_cast<size_t>(p.c.B) * p.c.Hkv * 2);
+  a.counts = reinterpret_cast<int32_t*>(a.cut_scale + pairs * 2);
+  a.holes = a.counts + pairs;
+  a.sources = a.holes + pairs * p.list;
   pa_status rc = p.c.D == 128 ? launch_evict_kind<128>(a, st) : launch_evict_kind<64>(a, st);
   scratch_free(own, st);
   return rc;
