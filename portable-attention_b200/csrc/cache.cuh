@@ -125,16 +125,74 @@ __device__ __forceinline__ uint32_t cache_enc2(float a, float b) {
   return static_cast<uint32_t>(x & 0xff) | (static_cast<uint32_t>(y & 0xff) << 8);
 }
 
-template <bool BF16>
-__device__ __forceinline__ float2 cache_unpack(uint32_t w) {
-  if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
-  return __half22float2(*reinterpret_cast<const __half2*>(&w));
-}
-
 // Largest finite magnitude of amax and x (NaN and infinities are passed over).
 __device__ __forceinline__ float cache_amax(float amax, float x) {
   const float m = fabsf(x);
   return m < INFINITY ? fmaxf(amax, m) : amax;
+}
+
+// Largest finite magnitude among 16 codes. Magnitudes compare as integers, two
+// 16-bit lanes at a time; only a NaN among them needs a closer look.
+template <int KIND>
+__device__ __forceinline__ float cache_absmax(const uint4& q) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  uint32_t m = 0u;
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    uint32_t x = w[i];
+    if (KIND == kCacheI8) {
+      const uint32_t neg = (x >> 7) & 0x01010101u;
+      x = (x ^ (neg * 0xffu)) + neg;  // |-128| is 0x80 and carries nowhere
+    } else {
+      x &= 0x7f7f7f7fu;
+    }
+    m = __vmaxu2(m, __vmaxu2(x & 0x00ff00ffu, (x >> 8) & 0x00ff00ffu));
+  }
+  const uint32_t top = (m & 0xffffu) > (m >> 16) ? (m & 0xffffu) : (m >> 16);
+  if (KIND == kCacheI8) return static_cast<float>(top);
+  if (top != 0x7fu) return cache_dec2<KIND>(top).x;
+  float f = 0.f;
+#pragma unroll 1
+  for (int i = 0; i < 16; ++i) f = cache_amax(f, cache_dec2<KIND>((w[i >> 2] >> (8 * (i & 3))) & 0xffu).x);
+  return f;
+}
+
+// Whether from / to is a power of two from 2^-14 to 2^15: codes then move between
+// the scales in fp16 arithmetic that rounds once.
+__device__ __forceinline__ bool cache_easy_ratio(float from, float to) {
+  const uint32_t a = __float_as_uint(from), b = __float_as_uint(to);
+  const int k = static_cast<int>(a >> 23) - static_cast<int>(b >> 23);
+  return ((a | b) & 0x807fffffu) == 0u && a != 0u && b != 0u && k >= -14 && k <= 15;
+}
+
+// Four codes times such a ratio, as codes. int8: 1536 + x rounds x to an integer
+// whose low byte is the code; products stay within the format where the new scale
+// fits them.
+template <int KIND>
+__device__ __forceinline__ uint32_t cache_rescale4(uint32_t w, __half2 ratio) {
+  if (KIND == kCacheE4M3) {
+    uint32_t o = 0u;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w >> (16 * i)) & 0xffffu), __NV_E4M3);
+      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), ratio);
+      o |= static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&x), __NV_SATFINITE, __NV_E4M3))
+           << (16 * i);
+    }
+    return o;
+  }
+  const uint32_t u = w ^ 0x80808080u;  // value + 128
+  const __half2 bias = __floats2half2_rn(1152.f, 1152.f), magic = __floats2half2_rn(1536.f, 1536.f);
+  uint32_t lo = __byte_perm(u, 0x64646464u, 0x4140), hi = __byte_perm(u, 0x64646464u, 0x4342);  // 1024 + that
+  const __half2 a = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&lo), bias), ratio, magic);
+  const __half2 b = __hfma2(__hsub2(*reinterpret_cast<const __half2*>(&hi), bias), ratio, magic);
+  return __byte_perm(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b), 0x6420);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float2 cache_unpack(uint32_t w) {
+  if (BF16) return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+  return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
 __device__ __forceinline__ float warp_max(float x) {

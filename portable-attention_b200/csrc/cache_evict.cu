@@ -167,31 +167,36 @@ __device__ __forceinline__ int4 warps_before(int x, int y, int (*warp_sum)[32]) 
                    __reduce_add_sync(0xffffffffu, u), __reduce_add_sync(0xffffffffu, v));
 }
 
-// Codes of a 16-byte piece under another scale, stored at p. A power of two
-// divides exactly as a product with its reciprocal.
-template <int KIND, bool POW2>
-__device__ __forceinline__ void recode(const uint4& q, float s, float to, float inv, uint8_t* p) {
+// 16 codes of scale s as codes of scale `to`: code * s / to, rounded once more.
+template <int KIND>
+__device__ __forceinline__ uint4 recode(const uint4& q, float s, float to) {
+  if (s == to) return q;
+  if (cache_easy_ratio(s, to)) {
+    const __half r = __float2half_rn(__fdividef(s, to));
+    const __half2 ratio = __halves2half2(r, r);
+    return make_uint4(cache_rescale4<KIND>(q.x, ratio), cache_rescale4<KIND>(q.y, ratio),
+                      cache_rescale4<KIND>(q.z, ratio), cache_rescale4<KIND>(q.w, ratio));
+  }
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   uint32_t o[4] = {0u, 0u, 0u, 0u};
-#pragma unroll
+#pragma unroll 1
   for (int e = 0; e < 8; ++e) {
     const float2 f = cache_dec2<KIND>(w[e >> 1] >> (16 * (e & 1)));
-    const float y = f.x * s, z = f.y * s;
-    o[e >> 1] |= (POW2 ? cache_enc2<KIND>(y * inv, z * inv) : cache_enc2<KIND>(__fdiv_rn(y, to), __fdiv_rn(z, to)))
-                 << (16 * (e & 1));
+    o[e >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x * s, to), __fdiv_rn(f.y * s, to)) << (16 * (e & 1));
   }
-  *reinterpret_cast<uint4*>(p) = make_uint4(o[0], o[1], o[2], o[3]);
+  return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
 // Moves into the scale block of rows lo.. of a cache's keys or values, by one
 // warp: places are taken 16 or 32 at a time, lane i looking up place i's source,
-// then rows are read in four rounds. One step stays in registers between the
+// then rows are read in kRounds rounds. One step stays in registers between the
 // maximum and the coding; larger blocks are read again.
-template <int KIND, int D>
+template <int KIND, int D, int kRounds>
 __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo) {
   constexpr int kPieces = D / 16;      // lanes per row
   constexpr int kRows = 32 / kPieces;  // rows per round of a warp
-  constexpr int kStep = 4 * kRows;     // places per step: 16 or 32
+  constexpr int kStep = kRounds * kRows < 32 ? kRounds * kRows : 32;  // places per step
+  static_assert(kStep == kRounds * kRows, "a lane for every place");
   const int lane = threadIdx.x & 31;
   const int bs = a.c.scale_block, n = a.budget;
   const int hi = lo + bs < n ? lo + bs : n;
@@ -227,10 +232,10 @@ __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, in
       }
     }
   };
-  uint4 x[4];
+  uint4 x[kRounds];
   auto read = [&]() {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRounds; ++u) {
       const int64_t f = __shfl_sync(0xffffffffu, from, u * kRows + lane / kPieces);
       x[u] = f >= 0 ? *reinterpret_cast<const uint4*>(cache + f + ch) : make_uint4(0u, 0u, 0u, 0u);
     }
@@ -240,54 +245,99 @@ __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, in
     look_up(first);
     read();
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRounds; ++u) {
       const float s = __shfl_sync(0xffffffffu, scale, u * kRows + lane / kPieces);
-      const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
-      float m = 0.f;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float2 f = cache_dec2<KIND>(w[e >> 1] >> (16 * (e & 1)));
-        m = cache_amax(cache_amax(m, f.x), f.y);
-      }
-      amax = cache_amax(amax, m * s);
+      amax = cache_amax(amax, cache_absmax<KIND>(x[u]) * s);
     }
   }
   const bool held = __any_sync(0xffffffffu, stays);
   const float need = cache_need_scale<KIND>(warp_max(amax));
   const float old = held ? was : 0.f;
   const float to = old > need ? old : need;
-  const bool pow2 = (__float_as_uint(to) & 0x807fffffu) == 0u;
-  const float inv = __fdiv_rn(1.f, to);
   for (int first = lo; first < hi; first += kStep) {
     if (hi - lo > kStep) {
       look_up(first);
       read();
     }
 #pragma unroll
-    for (int u = 0; u < 4; ++u) {
+    for (int u = 0; u < kRounds; ++u) {
       const int j = u * kRows + lane / kPieces;
       const int64_t f = __shfl_sync(0xffffffffu, from, j);
       const float s = __shfl_sync(0xffffffffu, scale, j);
-      if (f < 0) continue;
-      uint8_t* p = dst0 + (first + j - lo) * a.c.key_stride;
-      if (pow2)
-        recode<KIND, true>(x[u], s, to, inv, p);
-      else
-        recode<KIND, false>(x[u], s, to, inv, p);
+      if (f >= 0) *reinterpret_cast<uint4*>(dst0 + (first + j - lo) * a.c.key_stride) = recode<KIND>(x[u], s, to);
     }
   }
-  if (held && to != old) {
+  if (held && to != old)
     for (int r = lo + lane / kPieces; r < hi; r += kRows) {
       if (kept[r] != r) continue;
-      uint8_t* p = dst0 + (r - lo) * a.c.key_stride;
-      recode<KIND, false>(*reinterpret_cast<const uint4*>(p), old, to, inv, p);
+      uint4* p = reinterpret_cast<uint4*>(dst0 + (r - lo) * a.c.key_stride);
+      *p = recode<KIND>(*p, old, to);
     }
-  }
   __syncwarp();
   if (lane == 0) *sp = to;
 }
 
-// kThreads and kCtas bound the registers: 1024 threads, or four CTAs of up to 320
+// List entries a warp takes at a time.
+constexpr int move_entries(int kind) { return cache_8bit(kind) ? 8 : 32; }
+
+// Moves by list entries, by one warp: in 16 bits the rows of 32 entries; in 8 bits
+// the scale blocks, of the keys or the values, whose first hole is among eight
+// entries (more warps than blocks: the chain of look-ups is what takes the time).
+template <int KIND, int D, int kRounds>
+__device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair, int b, int h, int chunk, int kv,
+                                                int m) {
+  const int lane = threadIdx.x & 31;
+  const int32_t* holes = a.holes + pair * a.list;
+  const int k0 = chunk * move_entries(KIND), k = k0 + lane;
+  const int cnt = m - k0 < move_entries(KIND) ? m - k0 : move_entries(KIND);
+  if (cache_8bit(KIND)) {
+    const int bs = a.c.scale_block;
+    const int block = lane < cnt ? holes[k] / bs : -1;
+    const int prev = lane < cnt && k > 0 ? holes[k - 1] / bs : -1;
+    uint32_t leads = __ballot_sync(0xffffffffu, lane < cnt && block != prev);
+    while (leads) {
+      const int l = __ffs(leads) - 1;
+      leads &= leads - 1;
+      move_block<KIND, D, kRounds>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs);
+    }
+    return;
+  }
+  constexpr int kPieces = D / 8;       // lanes per row
+  constexpr int kRows = 32 / kPieces;  // rows per step of a warp
+  int64_t from = -1, to = -1;
+  if (lane < cnt) {
+    const int dst = holes[k], src = a.sources[pair * a.list + k];
+    const int32_t pd = cache_page(a.c, a.table, b, dst, a.status), ps = cache_page(a.c, a.table, b, src, a.status);
+    if (pd >= 0 && ps >= 0) {
+      to = cache_row(a.c, pd, h, cache_at(a.c, dst));
+      from = cache_row(a.c, ps, h, cache_at(a.c, src));
+    }
+  }
+  const int ch = (lane % kPieces) * 16;
+  for (int i = 0; i < cnt; i += 4 * kRows) {
+    uint4 x[4][2];
+    int64_t d[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = i + u * kRows + lane / kPieces;
+      const int64_t s = __shfl_sync(0xffffffffu, from, j & 31);
+      d[u] = __shfl_sync(0xffffffffu, to, j & 31);
+      if (j >= cnt) d[u] = -1;
+      if (d[u] >= 0) {
+        x[u][0] = *reinterpret_cast<const uint4*>(a.cache[0] + s + ch);
+        x[u][1] = *reinterpret_cast<const uint4*>(a.cache[1] + s + ch);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+      if (d[u] >= 0) {
+        *reinterpret_cast<uint4*>(a.cache[0] + d[u] + ch) = x[u][0];
+        *reinterpret_cast<uint4*>(a.cache[1] + d[u] + ch) = x[u][1];
+      }
+  }
+}
+
+// kThreads and kCtas bound the registers: 1024 threads, or four CTAs of 256 to 320
 // for many short sequences, so that 512 of them run at once.
 template <int kKeys, int kThreads, int kCtas>
 __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const EvictArgs a) {
@@ -308,6 +358,40 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   int32_t* kept = a.kept + pair * n;
   int32_t* holes = a.holes + pair * a.list;
   int32_t* sources = a.sources + pair * a.list;
+  constexpr int kGroups = kKeys / 4;
+  const int lane = tid & 31;
+  const int per_round = T * kKeys;
+  // A thread's rows of a round: group q is four rows from my_row + 128 q on.
+  int64_t my_row = 0;
+  float4 wv[kGroups];
+  int4 pv[kGroups];
+  auto fetch = [&](int64_t first, int64_t end) {
+    my_row = first + (tid >> 5) * (32 * kKeys) + lane * 4;
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      const int64_t r = my_row + q * 128;
+      const int r32 = static_cast<int>(r);
+      wv[q] = make_float4(0.f, 0.f, 0.f, 0.f);
+      pv[q] = make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
+      if (r + 4 <= end && a.vec) {
+        wv[q] = *reinterpret_cast<const float4*>(w + r);
+        if (pos) pv[q] = *reinterpret_cast<const int4*>(pos + r);
+      } else if (r < end) {
+        wv[q].x = w[r];
+        if (r + 1 < end) wv[q].y = w[r + 1];
+        if (r + 2 < end) wv[q].z = w[r + 2];
+        if (r + 3 < end) wv[q].w = w[r + 3];
+        if (pos) {
+          pv[q].x = pos[r];
+          if (r + 1 < end) pv[q].y = pos[r + 1];
+          if (r + 2 < end) pv[q].z = pos[r + 2];
+          if (r + 3 < end) pv[q].w = pos[r + 3];
+        }
+      }
+    }
+  };
+  // One CTA's first rows do not depend on the length: asked for together with it.
+  if (C == 1) fetch(0, a.c.max_len);
   const bool bad = len < 0 || len > a.c.max_len;
   if (h == 0 && rank == 0 && tid == 0) {
     if (bad) atomicExch(a.status, kStatusBadSeqLen);
@@ -333,57 +417,67 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   const int share = ((len + C - 1) / C + 3) / 4 * 4;
   const int64_t row0 = static_cast<int64_t>(rank) * share;
   const int64_t row_end = row0 + share < len ? row0 + share : len;
-  const int per_round = T * kKeys;
   const int rounds = (share + per_round - 1) / per_round;
   const int64_t next = a.next ? a.next[b] : len;
   const int64_t newest = next - a.recent;
-  constexpr int kGroups = kKeys / 4;
-  const int lane = tid & 31;
   uint32_t keys[kKeys];
-  uint32_t live = 0;   // rows this thread holds in the current round
-  int64_t my_row = 0;  // the first of them; group q starts 128 q further on
+  uint32_t live = 0;  // rows this thread holds in the current round
   auto row_of = [&](int i) { return my_row + (i / 4) * 128 + (i & 3); };
-  auto load_keys = [&](int round) {
-    my_row = row0 + static_cast<int64_t>(round) * per_round + (tid >> 5) * (32 * kKeys) + lane * 4;
+  auto rank_keys = [&]() {
     live = 0;
-    float4 wv[kGroups];
-    int4 pv[kGroups];
-#pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
-      const int64_t r = my_row + q * 128;
-      wv[q] = make_float4(0.f, 0.f, 0.f, 0.f);
-      pv[q] = make_int4(0, 0, 0, 0);
-      if (r + 4 <= row_end && a.vec) {
-        wv[q] = *reinterpret_cast<const float4*>(w + r);
-        if (pos) pv[q] = *reinterpret_cast<const int4*>(pos + r);
-        live |= 15u << (4 * q);
-      } else if (r < row_end) {
-        float* wf = &wv[q].x;
-        int* pf = &pv[q].x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (r + e < row_end) {
-            wf[e] = w[r + e];
-            if (pos) pf[e] = pos[r + e];
-            live |= 1u << (4 * q + e);
-          }
-      }
-    }
 #pragma unroll
     for (int q = 0; q < kGroups; ++q) {
       const float wf[4] = {wv[q].x, wv[q].y, wv[q].z, wv[q].w};
       const int pf[4] = {pv[q].x, pv[q].y, pv[q].z, pv[q].w};
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const int64_t p = pos ? pf[e] : my_row + q * 128 + e;
-        keys[4 * q + e] = p >= newest || p < a.sinks ? 0xffffffffu : weight_key(wf[e]);
+        live |= row_of(4 * q + e) < row_end ? 1u << (4 * q + e) : 0u;
+        keys[4 * q + e] = pf[e] >= newest || pf[e] < a.sinks ? 0xffffffffu : weight_key(wf[e]);
+      }
+    }
+  };
+  auto load_keys = [&](int round) {
+    fetch(row0 + static_cast<int64_t>(round) * per_round, row_end);
+    rank_keys();
+  };
+  // kept[] below the budget as if every row stayed, and weights and positions too
+  // (a cluster's few CTAs with such rows leave that to the end); places that
+  // receive rows are written again.
+  auto copy_rows = [&]() {
+    const bool copy_w = C == 1 && w_out && w_out != w, copy_p = C == 1 && p_out && p_out != pos;
+    const int64_t end = row_end < n ? row_end : n;
+#pragma unroll
+    for (int q = 0; q < kGroups; ++q) {
+      const int64_t r = my_row + q * 128;
+      const int r32 = static_cast<int>(r);
+      if (r + 4 <= end && a.vec) {
+        if (copy_w) *reinterpret_cast<float4*>(w_out + r) = wv[q];
+        if (copy_p) *reinterpret_cast<int4*>(p_out + r) = pv[q];
+      } else {
+        const float wf[4] = {wv[q].x, wv[q].y, wv[q].z, wv[q].w};
+        const int pf[4] = {pv[q].x, pv[q].y, pv[q].z, pv[q].w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          if (r + e < end && copy_w) w_out[r + e] = wf[e];
+          if (r + e < end && copy_p) p_out[r + e] = pf[e];
+        }
+      }
+      if (r + 4 <= end && a.vec_kept) {
+        *reinterpret_cast<int4*>(kept + r) = make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (r + e < end) kept[r + e] = r32 + e;
       }
     }
   };
 
   // ------------------------------------------------ threshold: radix selection
-  for (int i = tid; i < 4 * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
-  load_keys(0);
+  // A cluster's CTAs add into each other's arrays, so all are cleared up front.
+  for (int i = tid; i < (C > 1 ? 4 : 1) * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
+  if (C > 1) fetch(row0, row_end);
+  rank_keys();
+  copy_rows();
   sync_all();
   uint32_t prefix = 0;
   int left = n;  // rows to take among those that match the prefix
@@ -394,7 +488,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
     const int width = pass == 2 ? 10 : 11;
 #pragma unroll 1
     for (int round = 0; round < rounds; ++round) {
-      if (rounds > 1) load_keys(round);
+      if (pass > 0 ? rounds > 1 : round > 0) load_keys(round);
+      if (pass == 0 && round > 0) copy_rows();
 #pragma unroll
       for (int i = 0; i < kKeys; ++i)
         if ((live >> i & 1u) && (pass == 0 || (keys[i] >> (shift + width)) == (prefix >> (shift + width))))
@@ -412,6 +507,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
     sync_all();
     // Thread t < 256 takes bins 8 t' .. 8 t' + 7 from the top, t' = 255 - t.
     int bins[kBins / kScanThreads], sum = 0;
+    if (C == 1 && pass < 2)
+      for (int i = tid; i < kBins; i += T) sh.hist[pass + 1][i] = 0;
     if (tid < kScanThreads) {
       const int first = (kScanThreads - 1 - tid) * (kBins / kScanThreads);
 #pragma unroll
@@ -533,7 +630,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
     src_base = x.y;
     hole_all = x.z;
   }
-  const bool copy_w = w_out && w_out != w, copy_p = p_out && p_out != pos;
   {
     int ties = tie_base, n_hole = hole_base, n_src = src_base;
 #pragma unroll 1
@@ -550,32 +646,6 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
           if (src >> i & 1u) sources[sr++] = static_cast<int32_t>(row_of(i));
         }
       }
-      // Rows that stay.
-#pragma unroll
-      for (int q = 0; q < kGroups; ++q) {
-        const uint32_t stay = keep & ~src;
-        const int64_t r = my_row + q * 128;
-        if ((stay >> (4 * q) & 15u) == 15u && a.vec) {
-          const int32_t r32 = static_cast<int32_t>(r);
-          if (copy_w) *reinterpret_cast<float4*>(w_out + r) = *reinterpret_cast<const float4*>(w + r);
-          if (copy_p)
-            *reinterpret_cast<int4*>(p_out + r) =
-                pos ? *reinterpret_cast<const int4*>(pos + r) : make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
-          if (a.vec_kept)
-            *reinterpret_cast<int4*>(kept + r) = make_int4(r32, r32 + 1, r32 + 2, r32 + 3);
-          else
-#pragma unroll
-            for (int e = 0; e < 4; ++e) kept[r + e] = r32 + e;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (stay >> (4 * q + e) & 1u) {
-              kept[r + e] = static_cast<int32_t>(r + e);
-              if (copy_w) w_out[r + e] = w[r + e];
-              if (copy_p) p_out[r + e] = pos ? pos[r + e] : static_cast<int32_t>(r + e);
-            }
-        }
-      }
       n_hole += round_holes;
       n_src += round_src;
       if (C == 1) hole_all = n_hole;
@@ -585,8 +655,26 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   for (int k = rank * T + tid; k < hole_all; k += C * T) {
     const int d = holes[k], q = sources[k];
     kept[d] = q;
-    if (w_out) w_out[d] = w[q];
-    if (p_out) p_out[d] = pos ? pos[q] : q;
+    if (C == 1 && w_out) w_out[d] = w[q];
+    if (C == 1 && p_out) p_out[d] = pos ? pos[q] : q;
+  }
+  if (C > 1) {
+    // All CTAs of the cluster together: the rows below the budget are few CTAs' own.
+    cluster_sync();
+    for (int r = rank * T + tid; r < n; r += 2 * C * T) {
+      const int r2 = r + C * T < n ? r + C * T : r;
+      const int q = kept[r], q2 = kept[r2];
+      const float x = w[q], x2 = w[q2];
+      const int32_t y = pos ? pos[q] : q, y2 = pos ? pos[q2] : q2;
+      if (w_out) {
+        w_out[r] = x;
+        w_out[r2] = x2;
+      }
+      if (p_out) {
+        p_out[r] = y;
+        p_out[r2] = y2;
+      }
+    }
   }
   if (rank == 0 && tid == 0) a.counts[pair] = hole_all;
   if (cache_8bit(a.c.kind) && rank == 0 && tid < 2 && n % a.c.scale_block) {
@@ -595,14 +683,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   }
 }
 
-// 16 bits: a warp moves the rows of 32 list entries. 8 bits: where moves can be as
-// many as blocks, a warp has one block's keys or values; where they are fewer, it
-// looks at eight entries and moves the scale blocks whose first hole is among
-// them. The chain of look-ups is what takes the time, hence the many warps.
-constexpr int move_entries(int kind) { return cache_8bit(kind) ? 8 : 32; }
-
-template <int KIND, int D>
-__global__ void __launch_bounds__(256, 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
+// The rows of 8-bit caches where moves can be as many as blocks: a warp has one
+// block's keys or values. Else by list entries.
+template <int KIND, int D, int kRounds>
+__global__ void __launch_bounds__(256, kRounds > 4 ? 3 : 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
   int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
   if (item >= items) return;
   const int lane = threadIdx.x & 31;
@@ -611,67 +695,18 @@ __global__ void __launch_bounds__(256, 4) cache_move_kernel(const EvictArgs a, i
   const int64_t pair = item / chunks;
   const int chunk = static_cast<int>(item % chunks);
   const int h = static_cast<int>(pair % a.c.Hkv), b = static_cast<int>(pair / a.c.Hkv);
-  const int32_t* holes = a.holes + pair * a.list;
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int m = a.counts[pair];
-  if (cache_8bit(KIND) && a.by_block) {
-    const int lo = chunk * a.c.scale_block;
-    const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
-    bool moved = false;
-    if (m > 0)
-      for (int r = lo + lane; r < hi; r += 32) moved = moved || a.kept[pair * a.budget + r] != r;
-    if (__any_sync(0xffffffffu, moved)) move_block<KIND, D>(a, kv, b, h, pair, lo);
+  if (m == 0) return;
+  if (!cache_8bit(KIND) || !a.by_block) {
+    if (chunk * move_entries(KIND) < m) move_entries_of<KIND, D, kRounds>(a, pair, b, h, chunk, kv, m);
     return;
   }
-  const int k0 = chunk * move_entries(KIND);
-  if (k0 >= m) return;
-  const int k = k0 + lane;
-  const int cnt = m - k0 < move_entries(KIND) ? m - k0 : move_entries(KIND);
-  if (cache_8bit(KIND)) {
-    const int bs = a.c.scale_block;
-    const int block = lane < cnt ? holes[k] / bs : -1;
-    const int prev = lane < cnt && k > 0 ? holes[k - 1] / bs : -1;
-    uint32_t leads = __ballot_sync(0xffffffffu, lane < cnt && block != prev);
-    while (leads) {
-      const int l = __ffs(leads) - 1;
-      leads &= leads - 1;
-      move_block<KIND, D>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs);
-    }
-  } else {
-    constexpr int kPieces = D / 8;       // lanes per row
-    constexpr int kRows = 32 / kPieces;  // rows per step of a warp
-    int64_t from = -1, to = -1;
-    if (lane < cnt) {
-      const int dst = holes[k], src = a.sources[pair * a.list + k];
-      const int32_t pd = cache_page(a.c, a.table, b, dst, a.status), ps = cache_page(a.c, a.table, b, src, a.status);
-      if (pd >= 0 && ps >= 0) {
-        to = cache_row(a.c, pd, h, cache_at(a.c, dst));
-        from = cache_row(a.c, ps, h, cache_at(a.c, src));
-      }
-    }
-    const int ch = (lane % kPieces) * 16;
-    for (int i = 0; i < cnt; i += 4 * kRows) {
-      uint4 x[4][2];
-      int64_t d[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) {
-        const int j = i + u * kRows + lane / kPieces;
-        const int64_t s = __shfl_sync(0xffffffffu, from, j & 31);
-        d[u] = __shfl_sync(0xffffffffu, to, j & 31);
-        if (j >= cnt) d[u] = -1;
-        if (d[u] >= 0) {
-          x[u][0] = *reinterpret_cast<const uint4*>(a.cache[0] + s + ch);
-          x[u][1] = *reinterpret_cast<const uint4*>(a.cache[1] + s + ch);
-        }
-      }
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-        if (d[u] >= 0) {
-          *reinterpret_cast<uint4*>(a.cache[0] + d[u] + ch) = x[u][0];
-          *reinterpret_cast<uint4*>(a.cache[1] + d[u] + ch) = x[u][1];
-        }
-    }
-  }
+  const int lo = chunk * a.c.scale_block;
+  const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
+  bool moved = false;
+  for (int r = lo + lane; r < hi; r += 32) moved = moved || a.kept[pair * a.budget + r] != r;
+  if (__any_sync(0xffffffffu, moved)) move_block<KIND, D, kRounds>(a, kv, b, h, pair, lo);
 }
 
 struct EvictPlan {
@@ -692,14 +727,16 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
   return PA_OK;
 }
 
-// A CTA per (sequence, kv head), or a cluster of 2, 4 or 8 while that leaves SMs
-// without work and every CTA 2048 rows; threads for eight rows each, sixteen
-// where 1024 threads of eight would need a second round.
+// A CTA per (sequence, kv head), or a cluster of 2, 4 or 8 while each CTA then has
+// an SM and 2048 rows (128 heads of 8191 rows: 44.0 us alone, 49.0 in pairs); threads for eight rows each, sixteen
+// where 1024 threads of eight would need a second round. (Carrying few moves over
+// in the same CTA instead of a second launch measured the same, 22.5 us for one
+// row of 2049 in 512 heads.)
 template <int KIND, int D>
 pa_status launch_evict(EvictArgs a, cudaStream_t st) {
   const int64_t pairs = static_cast<int64_t>(a.c.B) * a.c.Hkv;
   int cluster = 1;
-  while (cluster < kMaxCluster && pairs * cluster * 2 <= 2 * sm_count() && a.c.max_len / (2 * cluster) >= 2048) cluster *= 2;
+  while (cluster < kMaxCluster && pairs * cluster * 2 <= sm_count() && a.c.max_len / (2 * cluster) >= 2048) cluster *= 2;
   a.cluster = cluster;
   const int64_t share = (static_cast<int64_t>(a.c.max_len) + cluster - 1) / cluster;
   const int keys = share > 8 * kMaxThreads ? 16 : 8;
@@ -735,7 +772,10 @@ pa_status launch_evict(EvictArgs a, cudaStream_t st) {
   cfg.gridDim = dim3(static_cast<unsigned>((items + 7) / 8));
   cfg.blockDim = dim3(256);
   cfg.dynamicSmemBytes = 0;
-  PA_CUDA(cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D>, a, chunks, items));
+  // Blocks of more than 16 rows of 128 bytes want eight rounds to stay in registers.
+  constexpr int kMany = cache_8bit(KIND) && D == 128 ? 8 : 4;
+  PA_CUDA(a.c.scale_block > 16 ? cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D, kMany>, a, chunks, items)
+                               : cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D, 4>, a, chunks, items));
   return PA_OK;
 }
 
