@@ -131,12 +131,19 @@ __device__ __forceinline__ float cache_amax(float amax, float x) {
   return m < INFINITY ? fmaxf(amax, m) : amax;
 }
 
+__device__ __forceinline__ uint32_t max_u16x2(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+  return d;
+}
+
 // Largest finite magnitude among 16 codes. Magnitudes compare as integers, two
-// 16-bit lanes at a time; only a NaN among them needs a closer look.
+// 16-bit lanes at a time (a lane's high byte decides); only a NaN among them needs
+// a closer look.
 template <int KIND>
 __device__ __forceinline__ float cache_absmax(const uint4& q) {
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-  uint32_t m = 0u;
+  uint32_t odd = 0u, even = 0u;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     uint32_t x = w[i];
@@ -146,9 +153,11 @@ __device__ __forceinline__ float cache_absmax(const uint4& q) {
     } else {
       x &= 0x7f7f7f7fu;
     }
-    m = __vmaxu2(m, __vmaxu2(x & 0x00ff00ffu, (x >> 8) & 0x00ff00ffu));
+    odd = max_u16x2(odd, x);
+    even = max_u16x2(even, __byte_perm(x, 0u, 0x2404));
   }
-  const uint32_t top = (m & 0xffffu) > (m >> 16) ? (m & 0xffffu) : (m >> 16);
+  const uint32_t m = max_u16x2(odd, even);
+  const uint32_t top = (m >> 24) > ((m >> 8) & 0xffu) ? m >> 24 : (m >> 8) & 0xffu;
   if (KIND == kCacheI8) return static_cast<float>(top);
   if (top != 0x7fu) return cache_dec2<KIND>(top).x;
   float f = 0.f;
@@ -165,21 +174,41 @@ __device__ __forceinline__ bool cache_easy_ratio(float from, float to) {
   return ((a | b) & 0x807fffffu) == 0u && a != 0u && b != 0u && k >= -14 && k <= 15;
 }
 
+// Four fp16 values as e4m3 codes (first in the low byte), and four codes as fp16.
+__device__ __forceinline__ uint32_t e4m3_from_h4(uint32_t a, uint32_t b) {
+  uint32_t d;
+  asm("{\n\t.reg .b16 l, h;\n\tcvt.rn.satfinite.e4m3x2.f16x2 l, %1;\n\tcvt.rn.satfinite.e4m3x2.f16x2 h, %2;\n\t"
+      "mov.b32 %0, {l, h};\n\t}"
+      : "=r"(d)
+      : "r"(a), "r"(b));
+  return d;
+}
+__device__ __forceinline__ void e4m3_to_h4(uint32_t w, uint32_t& a, uint32_t& b) {
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, l;\n\tcvt.rn.f16x2.e4m3x2 %1, h;\n\t}"
+      : "=r"(a), "=r"(b)
+      : "r"(w));
+}
+__device__ __forceinline__ uint32_t h2_mul(uint32_t a, __half2 b) {
+  const __half2 p = __hmul2(*reinterpret_cast<const __half2*>(&a), b);
+  return *reinterpret_cast<const uint32_t*>(&p);
+}
+
+// That ratio, twice.
+__device__ __forceinline__ __half2 cache_ratio(float from, float to) {
+  const uint32_t k = (__float_as_uint(from) >> 23) - (__float_as_uint(to) >> 23) + 15u;
+  const uint32_t h = (k << 10) | (k << 26);
+  return *reinterpret_cast<const __half2*>(&h);
+}
+
 // Four codes times such a ratio, as codes. int8: 1536 + x rounds x to an integer
 // whose low byte is the code; products stay within the format where the new scale
 // fits them.
 template <int KIND>
 __device__ __forceinline__ uint32_t cache_rescale4(uint32_t w, __half2 ratio) {
   if (KIND == kCacheE4M3) {
-    uint32_t o = 0u;
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>((w >> (16 * i)) & 0xffffu), __NV_E4M3);
-      const __half2 x = __hmul2(*reinterpret_cast<const __half2*>(&h), ratio);
-      o |= static_cast<uint32_t>(__nv_cvt_halfraw2_to_fp8x2(*reinterpret_cast<const __half2_raw*>(&x), __NV_SATFINITE, __NV_E4M3))
-           << (16 * i);
-    }
-    return o;
+    uint32_t a, b;
+    e4m3_to_h4(w, a, b);
+    return e4m3_from_h4(h2_mul(a, ratio), h2_mul(b, ratio));
   }
   const uint32_t u = w ^ 0x80808080u;  // value + 128
   const __half2 bias = __floats2half2_rn(1152.f, 1152.f), magic = __floats2half2_rn(1536.f, 1536.f);

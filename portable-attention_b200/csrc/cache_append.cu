@@ -10,7 +10,11 @@
 //
 // One warp owns one (sequence, block, kv head, K or V), so a scale has one
 // writer and its rows need no other synchronisation. Lanes take 16-byte pieces
-// (8 elements) of consecutive rows.
+// (8 elements) of consecutive rows. Up to eight pieces a lane (16 rows of 128, 32
+// of 64) stay in registers between the maximum and the coding, so the input is
+// read once; larger blocks are read again. Magnitudes compare as integers two at
+// a time, and where s' is a power of two in fp16's range the coding is packed
+// fp16 arithmetic that rounds once: about 0.15 instructions a thread and element.
 #include <math.h>
 
 #include <cmath>
@@ -129,8 +133,48 @@ struct AppendArgs {
   int64_t items;
 };
 
-template <int KIND, int D, bool QBF16>
-__global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
+// Eight 16-bit elements as codes of scale s. EASY: s is a power of two whose
+// reciprocal fp16 holds as a normal number, and every element is finite.
+template <int KIND, bool QBF16, bool EASY>
+__device__ __forceinline__ uint2 encode8(const uint4& q, float s, float inv) {
+  const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+  if constexpr (EASY && !QBF16 && KIND == kCacheE4M3) {
+    const __half r = __float2half_rn(inv);
+    const __half2 r2 = __halves2half2(r, r);
+    return make_uint2(e4m3_from_h4(h2_mul(w[0], r2), h2_mul(w[1], r2)),
+                      e4m3_from_h4(h2_mul(w[2], r2), h2_mul(w[3], r2)));
+  } else if constexpr (EASY && !QBF16) {
+    const __half r = __float2half_rn(inv);
+    const __half2 r2 = __halves2half2(r, r);
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {  // 1536 + x rounds to an integer whose low byte is the code
+      const __half2 y = __hfma2(*reinterpret_cast<const __half2*>(&w[k]), r2, __floats2half2_rn(1536.f, 1536.f));
+      o[k] = *reinterpret_cast<const uint32_t*>(&y);
+    }
+    return make_uint2(__byte_perm(o[0], o[1], 0x6420), __byte_perm(o[2], o[3], 0x6420));
+  } else {
+    uint32_t o[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float2 f = cache_unpack<QBF16>(w[k]);
+      if (EASY && KIND == kCacheI8) {
+        const float x = fmaf(f.x, inv, 12582912.f), y = fmaf(f.y, inv, 12582912.f);  // 1.5 * 2^23
+        o[k] = __byte_perm(__float_as_uint(x), __float_as_uint(y), 0x0040);
+      } else if (EASY) {
+        o[k] = cache_enc2<KIND>(f.x * inv, f.y * inv);
+      } else {
+        o[k] = cache_enc2<KIND>(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s));
+      }
+    }
+    return make_uint2(__byte_perm(o[0], o[1], 0x5410), __byte_perm(o[2], o[3], 0x5410));
+  }
+}
+
+// kHold: pieces a lane holds, eight, or four for blocks that have no more (eight
+// rows of 128: 65.7 us with eight, 55.5 with four, for 8 x 4096 tokens).
+template <int KIND, int D, bool QBF16, int kHold>
+__global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(const AppendArgs a) {
   const int lane = threadIdx.x & 31;
   const int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
   if (item >= a.items) return;
@@ -156,25 +200,49 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const int lo = r0 > len ? r0 : len;  // first new row
   const int hi = static_cast<int>(r_first + bs < static_cast<int64_t>(len) + add ? r_first + bs : len + add);
 
-  if (kv == 0 && (a.weights || a.positions)) {
+  constexpr int kChunks = D / 8;       // 16-byte pieces of a new row
+  constexpr int kRows = 32 / kChunks;  // rows per step of the warp
+  const int row_l = lane / kChunks, ch = lane % kChunks;
+  // This lane's piece of row lo + row_l; its next is kRows rows on.
+  const uint8_t* const src =
+      (kv ? a.x[1] : a.x[0]) + b * a.x_seq + h * a.x_head + (lo - len + row_l) * a.x_tok + ch * 16;
+  uint8_t* const cache = kv ? a.cache[1] : a.cache[0];
+  const int rows = hi - lo;
+  auto set_rows = [&]() {
+    if (kv != 0 || !(a.weights || a.positions)) return;
     const int64_t row0 = b * a.c.row_seq + h * a.c.row_head;
-    const int p0 = a.start ? a.start[b] : len;
+    const int p0 = a.positions ? (a.start ? a.start[b] : len) : 0;
     for (int r = lo + lane; r < hi; r += 32) {
       if (a.weights) a.weights[row0 + r] = 0.f;
       if (a.positions) a.positions[row0 + r] = p0 + (r - len);
     }
-  }
-  constexpr int kChunks = D / 8;  // 16-byte pieces of a new row
-  const uint8_t* src = a.x[kv] + b * a.x_seq + h * a.x_head;
-  const int n = (hi - lo) * kChunks;
+  };
 
+  uint4 x[kHold];
+  const int64_t x_step = kRows * a.x_tok;
+  auto read = [&](int first) {
+    const uint8_t* p = src + first * a.x_tok;
+    if (rows - first >= kHold * kRows) {
+#pragma unroll
+      for (int u = 0; u < kHold; ++u, p += x_step) x[u] = __ldcs(reinterpret_cast<const uint4*>(p));
+      return;
+    }
+#pragma unroll
+    for (int u = 0; u < kHold; ++u, p += x_step) {
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      if (first + u * kRows + row_l < rows) x[u] = __ldcs(reinterpret_cast<const uint4*>(p));
+    }
+  };
+  read(0);  // asked for before the page is known
+  set_rows();
   if (!cache_8bit(KIND)) {
-    for (int i = lane; i < n; i += 32) {
-      const int r = lo + i / kChunks, ch = i % kChunks;
-      const int32_t page = cache_page(a.c, a.table, b, r, a.status);
+#pragma unroll
+    for (int u = 0; u < kHold; ++u) {
+      const int i = u * kRows + row_l;
+      if (i >= rows) continue;
+      const int32_t page = cache_page(a.c, a.table, b, lo + i, a.status);
       if (page < 0) continue;
-      const uint4 w = *reinterpret_cast<const uint4*>(src + (r - len) * a.x_tok + ch * 16);
-      *reinterpret_cast<uint4*>(a.cache[kv] + cache_row(a.c, page, h, cache_at(a.c, r)) + ch * 16) = w;
+      *reinterpret_cast<uint4*>(cache + cache_row(a.c, page, h, cache_at(a.c, lo + i)) + ch * 16) = x[u];
     }
     return;
   }
@@ -182,40 +250,81 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
   const int32_t page = cache_page(a.c, a.table, b, lo, a.status);
   if (page < 0) return;
   const int at0 = cache_at(a.c, r0);  // the block's first row inside its page
-  float amax = 0.f;
-  for (int i = lane; i < n; i += 32) {
-    const uint4 w = *reinterpret_cast<const uint4*>(src + (lo + i / kChunks - len) * a.x_tok + (i % kChunks) * 16);
-    const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = cache_unpack<QBF16>(wd[k]);
-      amax = cache_amax(cache_amax(amax, f.x), f.y);
-    }
-  }
-  amax = warp_max(amax);
-  float* sp = a.scales[kv] + cache_scale(a.c, page, h, at0);
+  float* const sp = (kv ? a.scales[1] : a.scales[0]) + cache_scale(a.c, page, h, at0);
   const bool held = r0 < len;  // earlier rows of this sequence live in the block
-  const float need = cache_need_scale<KIND>(amax);
   const float old = held ? *sp : 0.f;
-  const float s = old > need ? old : need;
-  uint8_t* dst = a.cache[kv] + cache_row(a.c, page, h, at0);
-  for (int i = lane; i < n; i += 32) {
-    const int r = lo + i / kChunks, ch = i % kChunks;
-    const uint4 w = *reinterpret_cast<const uint4*>(src + (r - len) * a.x_tok + ch * 16);
-    const uint32_t wd[4] = {w.x, w.y, w.z, w.w};
-    uint32_t o[2] = {0u, 0u};
+  // Largest magnitude, as 16-bit patterns; a pattern of `inf` or above is not finite.
+  constexpr uint32_t kInf = QBF16 ? 0x7f80u : 0x7c00u;
+  uint32_t top = 0u;
+  for (int first = 0; first < rows; first += kHold * kRows) {
+    if (first > 0) read(first);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const float2 f = cache_unpack<QBF16>(wd[k]);
-      o[k >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x, s), __fdiv_rn(f.y, s)) << (16 * (k & 1));
+    for (int u = 0; u < kHold; ++u)
+      top = max_u16x2(max_u16x2(top, max_u16x2(x[u].x & 0x7fff7fffu, x[u].y & 0x7fff7fffu)),
+                      max_u16x2(x[u].z & 0x7fff7fffu, x[u].w & 0x7fff7fffu));
+  }
+  top = __reduce_max_sync(0xffffffffu, (top & 0xffffu) > (top >> 16) ? top & 0xffffu : top >> 16);
+  const bool finite = top < kInf;
+  float amax = cache_unpack<QBF16>(top).x;
+  if (!finite) {  // look again, passing over what is not
+    amax = 0.f;
+    for (int first = 0; first < rows; first += kHold * kRows) {
+      if (rows > kHold * kRows) read(first);
+#pragma unroll
+      for (int u = 0; u < kHold; ++u) {
+        const uint32_t w[4] = {x[u].x, x[u].y, x[u].z, x[u].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+          const float2 f = cache_unpack<QBF16>(w[k]);
+          amax = cache_amax(cache_amax(amax, f.x), f.y);
+        }
+      }
     }
-    *reinterpret_cast<uint2*>(dst + (r - r0) * a.c.key_stride + ch * 8) = make_uint2(o[0], o[1]);
+    amax = warp_max(amax);
+  }
+  const float need = cache_need_scale<KIND>(amax);
+  const float s = old > need ? old : need;
+  // 2^-15 <= s <= 2^14, a power of two: its reciprocal is a normal fp16 number.
+  const bool easy = finite && cache_easy_ratio(1.f, s);
+  const float inv = __fdiv_rn(1.f, s);
+  uint8_t* const dst = cache + cache_row(a.c, page, h, at0) + ch * 8;
+  uint8_t* const dst_l = dst + (lo - r0 + row_l) * a.c.key_stride;
+  for (int first = 0; first < rows; first += kHold * kRows) {
+    if (rows > kHold * kRows) read(first);
+    if (easy) {
+      uint8_t* p = dst_l + first * a.c.key_stride;
+      const int64_t step = kRows * a.c.key_stride;
+      if (rows - first >= kHold * kRows) {
+#pragma unroll
+        for (int u = 0; u < kHold; ++u, p += step) *reinterpret_cast<uint2*>(p) = encode8<KIND, QBF16, true>(x[u], s, inv);
+      } else {
+#pragma unroll
+        for (int u = 0; u < kHold; ++u, p += step)
+          if (first + u * kRows + row_l < rows) *reinterpret_cast<uint2*>(p) = encode8<KIND, QBF16, true>(x[u], s, inv);
+      }
+    } else {
+#pragma unroll 1
+      for (int u = 0; u < kHold; ++u) {
+        const int i = first + u * kRows;
+        if (i + row_l < rows) {
+          const uint4 q = *reinterpret_cast<const uint4*>(src + i * a.x_tok);
+          *reinterpret_cast<uint2*>(dst_l + i * a.c.key_stride) = encode8<KIND, QBF16, false>(q, s, inv);
+        }
+      }
+    }
   }
   if (held && s != old) {
     // The scale grew: the block's earlier rows are coded again.
-    for (int i = lane; i < (len - r0) * kChunks; i += 32) {
-      uint2* p = reinterpret_cast<uint2*>(dst + (i / kChunks) * a.c.key_stride + (i % kChunks) * 8);
+    const bool quick = cache_easy_ratio(old, s);
+    const __half2 ratio = cache_ratio(old, s);
+#pragma unroll 1
+    for (int i = row_l; i < len - r0; i += kRows) {
+      uint2* p = reinterpret_cast<uint2*>(dst + i * a.c.key_stride);
       const uint2 w = *p;
+      if (quick) {
+        *p = make_uint2(cache_rescale4<KIND>(w.x, ratio), cache_rescale4<KIND>(w.y, ratio));
+        continue;
+      }
       const uint32_t wd[2] = {w.x, w.y};
       uint32_t o[2] = {0u, 0u};
 #pragma unroll
@@ -232,9 +341,10 @@ __global__ void __launch_bounds__(256) cache_append_kernel(const AppendArgs a) {
 
 template <int KIND, int D, bool QBF16>
 pa_status launch_append(const AppendArgs& a, cudaStream_t st) {
+  auto kern = a.rows_per_block * (D / 8) <= 4 * 32 ? cache_append_kernel<KIND, D, QBF16, 4> : cache_append_kernel<KIND, D, QBF16, 8>;
   const int64_t grid = (a.items + 7) / 8;
   if (grid > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache append: grid too large");
-  cache_append_kernel<KIND, D, QBF16><<<static_cast<unsigned>(grid), 256, 0, st>>>(a);
+  kern<<<static_cast<unsigned>(grid), 256, 0, st>>>(a);
   PA_CUDA(cudaGetLastError());
   return PA_OK;
 }
@@ -300,9 +410,11 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   a.x_tok = new_token_stride * 2;
   a.x_head = new_head_stride * 2;
   a.T = static_cast<int32_t>(new_len);
-  // 16-bit caches have no blocks: 16 rows make an item.
+  // 16-bit caches have no blocks: 16 rows make an item (eight pieces a lane, or four).
   a.rows_per_block = cache_8bit(a.c.kind) ? a.c.scale_block : 16;
-  a.blocks = a.T / a.rows_per_block + 2;  // blocks that T rows starting anywhere can touch
+  // Blocks that T rows starting anywhere can touch; one at least, for seq_lens_out.
+  const int64_t bs = a.rows_per_block;
+  a.blocks = a.T > 0 ? static_cast<int32_t>((a.T + 2 * bs - 2) / bs) : 1;
   a.items = static_cast<int64_t>(a.c.B) * a.blocks * 2 * a.c.Hkv;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return a.c.D == 128 ? launch_append_kind<128>(a, st) : launch_append_kind<64>(a, st);

@@ -169,17 +169,17 @@ __device__ __forceinline__ int4 warps_before(int x, int y, int (*warp_sum)[32]) 
 
 // 16 codes of scale s as codes of scale `to`: code * s / to, rounded once more.
 template <int KIND>
-__device__ __forceinline__ uint4 recode(const uint4& q, float s, float to) {
+__device__ __forceinline__ uint4 recode_easy(const uint4& q, float s, float to) {
+  const __half2 r = cache_ratio(s, to);
+  return make_uint4(cache_rescale4<KIND>(q.x, r), cache_rescale4<KIND>(q.y, r), cache_rescale4<KIND>(q.z, r),
+                    cache_rescale4<KIND>(q.w, r));
+}
+template <int KIND>
+__device__ __noinline__ uint4 recode(uint4 q, float s, float to) {
   if (s == to) return q;
-  if (cache_easy_ratio(s, to)) {
-    const __half r = __float2half_rn(__fdividef(s, to));
-    const __half2 ratio = __halves2half2(r, r);
-    return make_uint4(cache_rescale4<KIND>(q.x, ratio), cache_rescale4<KIND>(q.y, ratio),
-                      cache_rescale4<KIND>(q.z, ratio), cache_rescale4<KIND>(q.w, ratio));
-  }
   const uint32_t w[4] = {q.x, q.y, q.z, q.w};
   uint32_t o[4] = {0u, 0u, 0u, 0u};
-#pragma unroll 1
+#pragma unroll
   for (int e = 0; e < 8; ++e) {
     const float2 f = cache_dec2<KIND>(w[e >> 1] >> (16 * (e & 1)));
     o[e >> 1] |= cache_enc2<KIND>(__fdiv_rn(f.x * s, to), __fdiv_rn(f.y * s, to)) << (16 * (e & 1));
@@ -187,16 +187,26 @@ __device__ __forceinline__ uint4 recode(const uint4& q, float s, float to) {
   return make_uint4(o[0], o[1], o[2], o[3]);
 }
 
+// What a warp needs of up to 32 moves into a block.
+struct MoveSlot {
+  int64_t from;  // source row, bytes from the cache's base
+  float scale;   // the source's scale
+  int place;     // row in the block
+};
+constexpr int kMoveWarps = 8;
+
 // Moves into the scale block of rows lo.. of a cache's keys or values, by one
-// warp: places are taken 16 or 32 at a time, lane i looking up place i's source,
-// then rows are read in kRounds rounds. One step stays in registers between the
-// maximum and the coding; larger blocks are read again.
-template <int KIND, int D, int kRounds>
-__device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo) {
+// warp. Places are taken 32 at a time: lane i looks up place i's source, and the
+// moves among them are packed into `slots` (the warp's own shared memory), so that
+// rows that stay cost no lanes. Rows are then read in steps of four rounds; a
+// block of one step stays in registers between the maximum and the coding, larger
+// ones are read again.
+template <int KIND, int D>
+__device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo,
+                                           MoveSlot* slots) {
   constexpr int kPieces = D / 16;      // lanes per row
   constexpr int kRows = 32 / kPieces;  // rows per round of a warp
-  constexpr int kStep = kRounds * kRows < 32 ? kRounds * kRows : 32;  // places per step
-  static_assert(kStep == kRounds * kRows, "a lane for every place");
+  constexpr int kStep = 4 * kRows;     // rows per step: 16 or 32
   const int lane = threadIdx.x & 31;
   const int bs = a.c.scale_block, n = a.budget;
   const int hi = lo + bs < n ? lo + bs : n;
@@ -211,67 +221,87 @@ __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, in
   float* const sp = scales + cache_scale(a.c, page, h, at_lo);
   uint8_t* const dst0 = cache + cache_row(a.c, page, h, at_lo) + ch;
   const float was = *sp;
-  int64_t from = -1;   // place `lane`: its source row (-1: it stays, or a bad page)
-  float scale = 0.f;   // and the source's scale
   bool stays = false;  // some place keeps its row
-  auto look_up = [&](int first) {
-    from = -1;
-    scale = 0.f;
+  // Packs the moves of the 32 places from `first` on; returns their number.
+  auto look_up = [&](int first) -> int {
     const int r = first + lane;
-    if (lane < kStep && r < hi) {
-      const int src = kept[r];
-      if (src == r) {
-        stays = true;
-      } else {
-        const int32_t ps = cache_page(a.c, a.table, b, src, a.status);
-        if (ps >= 0) {
-          const int at = cache_at(a.c, src);
-          from = cache_row(a.c, ps, h, at);
-          scale = src / bs == cut ? a.cut_scale[pair * 2 + kv] : scales[cache_scale(a.c, ps, h, at)];
-        }
+    const int src = r < hi ? kept[r] : r;
+    MoveSlot m{-1, 0.f, r - lo};
+    if (src != r) {
+      const int32_t ps = cache_page(a.c, a.table, b, src, a.status);
+      if (ps >= 0) {
+        const int at = cache_at(a.c, src);
+        m.from = cache_row(a.c, ps, h, at);
+        m.scale = src / bs == cut ? a.cut_scale[pair * 2 + kv] : scales[cache_scale(a.c, ps, h, at)];
+      }
+    }
+    const uint32_t moves = __ballot_sync(0xffffffffu, m.from >= 0);
+    stays = stays || __any_sync(0xffffffffu, r < hi && src == r);
+    __syncwarp();  // the slots' last readers are done
+    if (m.from >= 0) slots[__popc(moves & ((1u << lane) - 1u))] = m;
+    __syncwarp();
+    return __popc(moves);
+  };
+  uint4 x[4];
+  float s[4];
+  int place[4];  // -1: nothing
+  auto read = [&](int first, int count) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = first + u * kRows + lane / kPieces;
+      x[u] = make_uint4(0u, 0u, 0u, 0u);
+      s[u] = 0.f;
+      place[u] = -1;
+      if (j < count) {
+        const MoveSlot m = slots[j];
+        x[u] = *reinterpret_cast<const uint4*>(cache + m.from + ch);
+        s[u] = m.scale;
+        place[u] = m.place;
       }
     }
   };
-  uint4 x[kRounds];
-  auto read = [&]() {
-#pragma unroll
-    for (int u = 0; u < kRounds; ++u) {
-      const int64_t f = __shfl_sync(0xffffffffu, from, u * kRows + lane / kPieces);
-      x[u] = f >= 0 ? *reinterpret_cast<const uint4*>(cache + f + ch) : make_uint4(0u, 0u, 0u, 0u);
-    }
-  };
   float amax = 0.f;
-  for (int first = lo; first < hi; first += kStep) {
-    look_up(first);
-    read();
+  int count = 0;
+  for (int first = lo; first < hi; first += 32) {
+    count = look_up(first);
+    for (int i = 0; i < count; i += kStep) {
+      read(i, count);
 #pragma unroll
-    for (int u = 0; u < kRounds; ++u) {
-      const float s = __shfl_sync(0xffffffffu, scale, u * kRows + lane / kPieces);
-      amax = cache_amax(amax, cache_absmax<KIND>(x[u]) * s);
+      for (int u = 0; u < 4; ++u) amax = cache_amax(amax, cache_absmax<KIND>(x[u]) * s[u]);
     }
   }
-  const bool held = __any_sync(0xffffffffu, stays);
   const float need = cache_need_scale<KIND>(warp_max(amax));
-  const float old = held ? was : 0.f;
+  const float old = stays ? was : 0.f;
   const float to = old > need ? old : need;
-  for (int first = lo; first < hi; first += kStep) {
-    if (hi - lo > kStep) {
-      look_up(first);
-      read();
-    }
+  const bool again = hi - lo > 32 || count > kStep;
+  for (int first = lo; first < hi; first += 32) {
+    if (hi - lo > 32) count = look_up(first);
+    for (int i = 0; i < count; i += kStep) {
+      if (again) read(i, count);
+      bool easy = true;
 #pragma unroll
-    for (int u = 0; u < kRounds; ++u) {
-      const int j = u * kRows + lane / kPieces;
-      const int64_t f = __shfl_sync(0xffffffffu, from, j);
-      const float s = __shfl_sync(0xffffffffu, scale, j);
-      if (f >= 0) *reinterpret_cast<uint4*>(dst0 + (first + j - lo) * a.c.key_stride) = recode<KIND>(x[u], s, to);
+      for (int u = 0; u < 4; ++u) easy = easy && (place[u] < 0 || cache_easy_ratio(s[u], to));
+      if (__all_sync(0xffffffffu, easy)) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          if (place[u] >= 0)
+            *reinterpret_cast<uint4*>(dst0 + place[u] * a.c.key_stride) = recode_easy<KIND>(x[u], s[u], to);
+      } else {
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+          const int p = u == 0 ? place[0] : u == 1 ? place[1] : u == 2 ? place[2] : place[3];
+          const float f = u == 0 ? s[0] : u == 1 ? s[1] : u == 2 ? s[2] : s[3];
+          const uint4 q = u == 0 ? x[0] : u == 1 ? x[1] : u == 2 ? x[2] : x[3];
+          if (p >= 0) *reinterpret_cast<uint4*>(dst0 + p * a.c.key_stride) = recode<KIND>(q, f, to);
+        }
+      }
     }
   }
-  if (held && to != old)
+  if (stays && to != old)
     for (int r = lo + lane / kPieces; r < hi; r += kRows) {
       if (kept[r] != r) continue;
       uint4* p = reinterpret_cast<uint4*>(dst0 + (r - lo) * a.c.key_stride);
-      *p = recode<KIND>(*p, old, to);
+      *p = cache_easy_ratio(old, to) ? recode_easy<KIND>(*p, old, to) : recode<KIND>(*p, old, to);
     }
   __syncwarp();
   if (lane == 0) *sp = to;
@@ -283,9 +313,9 @@ constexpr int move_entries(int kind) { return cache_8bit(kind) ? 8 : 32; }
 // Moves by list entries, by one warp: in 16 bits the rows of 32 entries; in 8 bits
 // the scale blocks, of the keys or the values, whose first hole is among eight
 // entries (more warps than blocks: the chain of look-ups is what takes the time).
-template <int KIND, int D, int kRounds>
+template <int KIND, int D>
 __device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair, int b, int h, int chunk, int kv,
-                                                int m) {
+                                                int m, MoveSlot* slots) {
   const int lane = threadIdx.x & 31;
   const int32_t* holes = a.holes + pair * a.list;
   const int k0 = chunk * move_entries(KIND), k = k0 + lane;
@@ -298,7 +328,7 @@ __device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair
     while (leads) {
       const int l = __ffs(leads) - 1;
       leads &= leads - 1;
-      move_block<KIND, D, kRounds>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs);
+      move_block<KIND, D>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs, slots);
     }
     return;
   }
@@ -685,8 +715,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
 
 // The rows of 8-bit caches where moves can be as many as blocks: a warp has one
 // block's keys or values. Else by list entries.
-template <int KIND, int D, int kRounds>
-__global__ void __launch_bounds__(256, kRounds > 4 ? 3 : 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
+template <int KIND, int D>
+__global__ void __launch_bounds__(32 * kMoveWarps, 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
+  __shared__ MoveSlot all_slots[kMoveWarps][32];
+  MoveSlot* const slots = all_slots[threadIdx.x >> 5];
   int64_t item = (blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x) >> 5;
   if (item >= items) return;
   const int lane = threadIdx.x & 31;
@@ -699,14 +731,14 @@ __global__ void __launch_bounds__(256, kRounds > 4 ? 3 : 4) cache_move_kernel(co
   const int m = a.counts[pair];
   if (m == 0) return;
   if (!cache_8bit(KIND) || !a.by_block) {
-    if (chunk * move_entries(KIND) < m) move_entries_of<KIND, D, kRounds>(a, pair, b, h, chunk, kv, m);
+    if (chunk * move_entries(KIND) < m) move_entries_of<KIND, D>(a, pair, b, h, chunk, kv, m, slots);
     return;
   }
   const int lo = chunk * a.c.scale_block;
   const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
   bool moved = false;
   for (int r = lo + lane; r < hi; r += 32) moved = moved || a.kept[pair * a.budget + r] != r;
-  if (__any_sync(0xffffffffu, moved)) move_block<KIND, D, kRounds>(a, kv, b, h, pair, lo);
+  if (__any_sync(0xffffffffu, moved)) move_block<KIND, D>(a, kv, b, h, pair, lo, slots);
 }
 
 struct EvictPlan {
@@ -764,18 +796,15 @@ pa_status launch_evict(EvictArgs a, cudaStream_t st) {
     if (a.by_block) chunks = blocks;
   }
   const int64_t items = pairs * chunks * (cache_8bit(KIND) ? 2 : 1);
-  if ((items + 7) / 8 > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
+  if (items / kMoveWarps >= 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
   // Starts while `select` ends; waits for its memory.
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
   cfg.numAttrs = 1;
-  cfg.gridDim = dim3(static_cast<unsigned>((items + 7) / 8));
-  cfg.blockDim = dim3(256);
+  cfg.gridDim = dim3(static_cast<unsigned>((items + kMoveWarps - 1) / kMoveWarps));
+  cfg.blockDim = dim3(32 * kMoveWarps);
   cfg.dynamicSmemBytes = 0;
-  // Blocks of more than 16 rows of 128 bytes want eight rounds to stay in registers.
-  constexpr int kMany = cache_8bit(KIND) && D == 128 ? 8 : 4;
-  PA_CUDA(a.c.scale_block > 16 ? cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D, kMany>, a, chunks, items)
-                               : cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D, 4>, a, chunks, items));
+  PA_CUDA(cudaLaunchKernelEx(&cfg, cache_move_kernel<KIND, D>, a, chunks, items));
   return PA_OK;
 }
 
