@@ -24,7 +24,8 @@
 // 2^(m_tile - m_run) * max|vs| * 2^-15. A probability down to 2^-29 of its tile's
 // largest keeps all 11 bits, whatever the other tiles hold: a first token that
 // takes nearly all the weight, as trained models have, costs the others nothing.
-// bf16 caches need bf16 products; there p' goes in as two bf16 terms.
+// bf16 caches need bf16 products; there p' has no factor (bf16 has the range, and
+// values near its end must not overflow the sums) and goes in as two bf16 terms.
 //
 // Splits leave (max, sum, accumulator) in the workspace and a second launch joins
 // them by log-sum-exp; a single split without weights writes its output itself.
@@ -45,7 +46,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxSplit = 512;
-constexpr float kPScale = 32768.f;
 constexpr float kMinScale = 7.52316385e-37f;  // 2^-120
 
 template <int KIND, int D, int HT>
@@ -185,6 +185,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
   constexpr bool kF8 = cache_8bit(KIND);
   constexpr bool kMmaBf16 = KIND == kCacheBF16;
   constexpr bool kTwo = HT == 16;
+  constexpr float kPScale = kMmaBf16 ? 1.f : 32768.f;
   constexpr int TK = C::kTK;
   constexpr int KS = D / 16;   // k-steps of Q K^T
   constexpr int MT = D / 16;   // m-tiles of V^T P^T
@@ -398,7 +399,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
 
     // ---- softmax of the tile: keys key_of(nt, e) of heads g (columns 0-1), g + 8 (2-3)
     auto key_of = [&](int nt, int e) { return kF8 ? 16 * (nt >> 1) + 4 * c + 2 * (nt & 1) + e : 8 * nt + 2 * c + e; };
-    float vw[NT][2];      // value scale over the tile's largest, times 2^15
+    float vw[NT][2];      // value scale over the tile's largest, times kPScale
     float vtile = 1.f / kPScale;
     if (kF8) {
       const float* sc = reinterpret_cast<const float*>(kt + C::kScaleOff);

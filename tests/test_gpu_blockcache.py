@@ -304,6 +304,28 @@ def test_evict_without_positions_and_with_equal_weights():
     assert list(got.seq_lens) == [40, 40]
 
 
+@pytest.mark.parametrize("fmt,B,H,n,budget,page,block", [
+    ("int8", 1, 1, 140001, 20003, 64, 64),     # a cluster whose threads hold their rows in two rounds
+    (None, 40, 2, 17001, 16990, 1024, 1024),   # one CTA a head, three rounds
+    (None, 2, 1, 70000, 69990, 1024, 1024), ("e4m3", 3, 2, 30000, 1000, 16, 16),
+])
+def test_evict_of_long_sequences(fmt, B, H, n, budget, page, block):
+    import pa_b200
+
+    rng = np.random.default_rng(n)
+    lens = np.array([n - 7 * (b % 3) for b in range(B)], np.int32)
+    c = Cache(rng, B, H, 64, page, block, fmt, lens, n)
+    w = np.exp(2 * rng.standard_normal((B, H, n))).astype(np.float32)
+    w[:, :, ::5] = np.float32(0.25)            # ties across threads, warps and rounds
+    got = pa_b200.cache_evict(seq_lens=lens, weights=w, budget=budget, recent=100, sinks=3, **c.arrays("hnd"))
+    want_w = w.copy()
+    want_len, kept = evict_reference(c.k, c.v, lens, want_w, budget, recent=100, sinks=3, fmt=fmt, **c.parts())
+    np.testing.assert_array_equal(got.kept, kept)
+    np.testing.assert_array_equal(got.weights, want_w)
+    np.testing.assert_array_equal(got.seq_lens, want_len)
+    c.check_equal(got, "hnd")
+
+
 def test_a_budgeted_serving_loop():
     """Prompt, then tokens: append, decode with weights, evict when over budget, against the oracle
     (which takes the device's own weights, so a close call in the choice cannot split the two)."""
@@ -480,6 +502,45 @@ def test_bf16_append_decode_evict_on_device_pointers(fmt, D, Hq, H, layout):
     np.testing.assert_array_equal(pos.cpu().numpy(), want_p)
     assert lens3.tolist() == list(want_len)
     d.check_equal()
+
+
+def test_bf16_cache_with_values_near_the_end_of_the_range():
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(17)
+    c = Cache(rng, 2, 1, 64, 16, 16, None, [40, 3], 48)
+    for x in (c.k, c.v):
+        x[:] = torch.from_numpy(x).to(torch.bfloat16).double().numpy()
+    c.v *= 2.0 ** 120                                   # up to about 5e36: finite in bf16 and fp32
+    d = OnDevice(c, "hnd", "bf16")
+    q = torch.from_numpy(rng.standard_normal((2, 4, 64))).to("cuda", torch.bfloat16)
+    out, lse = torch.empty_like(q), torch.empty((2, 4), device="cuda")
+    pa_b200.cache_decode_device(d.desc(4, 48, "bf16"), q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), out.data_ptr(),
+                                seq_lens_ptr=d.lens.data_ptr(), lse_ptr=lse.data_ptr(), **d.kw())
+    torch.cuda.synchronize()
+    pa_b200.sync_device_status()
+    ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, [40, 3], **c.parts())
+    check_decode(ref, out.double().cpu().numpy(), lse.cpu().numpy(), u=U["bf16"])
+
+
+def test_calls_with_an_empty_batch_no_tokens_and_no_rows():
+    import pa_b200
+
+    rng = np.random.default_rng(18)
+    c = Cache(rng, 2, 2, 64, 16, 16, "e4m3", [20, 0], 32)
+    a = c.arrays("hnd")
+    none = np.zeros((2, 0, 2, 64), np.float16)
+    got = pa_b200.cache_append(none, none, seq_lens=[20, 0], **a)
+    c.check_equal(got, "hnd")
+    assert list(got.seq_lens) == [20, 0]
+    got = pa_b200.cache_evict(seq_lens=[0, 0], weights=np.zeros((2, 2, 32), np.float32), budget=3, **a)
+    assert (got.kept == -1).all() and list(got.seq_lens) == [0, 0]
+    out, lse = pa_b200.cache_decode(np.ones((2, 4, 64), np.float16), seq_lens=[0, 0], return_lse=True, **a)
+    assert (out == 0).all() and np.isneginf(lse).all()
+    b = {**a, "block_table": a["block_table"][:0]}
+    assert pa_b200.cache_decode(np.ones((0, 4, 64), np.float16), seq_lens=np.zeros(0, np.int32), **b).shape == (0, 4, 64)
+    assert pa_b200.cache_append(none[:0], none[:0], seq_lens=np.zeros(0, np.int32), **b).seq_lens.shape == (0,)
 
 
 def test_a_step_captured_in_a_graph_and_two_graphs_at_once():
