@@ -744,7 +744,9 @@ struct DecodePlan {
   size_t bytes;
 };
 
-// Splits of a (sequence, kv head), by a model of the launch in microseconds:
+// Splits of a (sequence, kv head). Where eight of each do not fill the resident
+// CTAs, as many as do (one sequence of 131071 keys, 8 kv heads: 28 splits 78 us,
+// 55 67, 74 78). Else up to eight, by a model of the launch in microseconds:
 //   waves w = pairs * ns / resident CTAs; a last wave that fills a part f of the
 //   slots still takes max(f, 0.75) of a full one (the reads saturate the memory
 //   before all slots are taken), each wave costs its CTAs' start, merge and partial
@@ -754,25 +756,28 @@ struct DecodePlan {
 // Measured at 64 x 8 x 32768 x 128 e4m3: 1 split 838 us, 3 splits 679, 6 633; 16
 // sequences: 2 splits 205, 3 176, 4 225; 64 ragged sequences of up to 8191 keys
 // (int8, 2 kv heads of 64): 3 splits 37.3, 6 29.0.
-int64_t choose_splits(int64_t pairs, int64_t tiles, int64_t most, int64_t wave, bool weights) {
+int64_t choose_splits(int64_t pairs, int64_t tiles, int64_t wave, bool weights) {
+  const int64_t most = tiles / kWarps < 1 ? 1 : tiles / kWarps;  // four tiles a CTA, one a warp
   if (pairs < 1) return 1;
+  if (pairs * 8 < wave) {
+    const int64_t ns = wave / pairs < most ? wave / pairs : most;
+    return ns < kMaxSplit ? ns : kMaxSplit;
+  }
   constexpr double kTileBytes = 8192, kBandwidth = 6.5e6, kCtaRate = 27e3;  // bytes, bytes/us
-  int64_t top = 2 * wave / pairs > 8 ? 2 * wave / pairs : 8;
-  top = top < most ? top : most;
-  top = top < kMaxSplit ? top : kMaxSplit;
+  const int64_t top = most < 8 ? most : 8;
   const double total = static_cast<double>(pairs) * tiles * kTileBytes / kBandwidth;
-  auto cost = [&](int64_t ns) {
+  double cost[9], least = 0;
+  for (int64_t ns = 1; ns <= top; ++ns) {
     const double w = static_cast<double>(pairs * ns) / wave;
     const double full = std::floor(w), f = w - full;
     const double ineff = (full + (f > 1e-9 ? std::fmax(f, 0.75) : 0.0)) / w;
     const double chunk = static_cast<double>((tiles + ns - 1) / ns) * kTileBytes;
-    return std::fmax(total * ineff, std::ceil(w) * chunk / kCtaRate) + 6.0 * std::ceil(w) + (ns > 1 || weights ? 3.0 : 0.0);
-  };
-  double least = cost(1);
-  for (int64_t n = 2; n <= top; ++n) least = std::fmin(least, cost(n));
+    cost[ns] = std::fmax(total * ineff, std::ceil(w) * chunk / kCtaRate) + 6.0 * std::ceil(w) + (ns > 1 || weights ? 3.0 : 0.0);
+    least = ns == 1 ? cost[1] : std::fmin(least, cost[ns]);
+  }
   int64_t ns = top;
-  while (ns > 1 && cost(ns) > 1.06 * least) --ns;
-  return ns < 1 ? 1 : ns;
+  while (ns > 1 && cost[ns] > 1.06 * least) --ns;
+  return ns;
 }
 
 pa_status plan_decode(const pa_block_cache_desc* d, bool paged, bool weights, DecodePlan* p) {
@@ -795,8 +800,7 @@ pa_status plan_decode(const pa_block_cache_desc* d, bool paged, bool weights, De
   const int64_t pairs = static_cast<int64_t>(p->c.B) * p->c.Hkv;
   const int64_t tiles = (static_cast<int64_t>(p->c.max_len) + tk - 1) / tk;
   const int64_t wave = (p->G <= 8 ? 3 : 2) * static_cast<int64_t>(sm_count());
-  const int64_t most = tiles / kWarps < 1 ? 1 : tiles / kWarps;
-  int64_t ns = choose_splits(pairs, tiles, most, wave, weights);
+  int64_t ns = choose_splits(pairs, tiles, wave, weights);
   const int64_t per = (tiles + ns - 1) / ns;
   const int64_t chunk = per * tk;
   p->chunk = static_cast<int>(chunk < tk ? tk : chunk);

@@ -196,13 +196,14 @@ struct MoveSlot {
 constexpr int kMoveWarps = 8;
 
 // Moves into the scale block of rows lo.. of a cache's keys or values, by one
-// warp. Places are taken 32 at a time: lane i looks up place i's source, and the
+// warp; src0 is kept[lo + lane] (or lo + lane behind the block). Places are taken
+// 32 at a time: lane i looks up place i's source, and the
 // moves among them are packed into `slots` (the warp's own shared memory), so that
 // rows that stay cost no lanes. Rows are then read in steps of four rounds; a
 // block of one step stays in registers between the maximum and the coding, larger
 // ones are read again.
 template <int KIND, int D>
-__device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo,
+__device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, int h, int64_t pair, int lo, int src0,
                                            MoveSlot* slots) {
   constexpr int kPieces = D / 16;      // lanes per row
   constexpr int kRows = 32 / kPieces;  // rows per round of a warp
@@ -225,7 +226,7 @@ __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, in
   // Packs the moves of the 32 places from `first` on; returns their number.
   auto look_up = [&](int first) -> int {
     const int r = first + lane;
-    const int src = r < hi ? kept[r] : r;
+    const int src = first == lo ? src0 : r < hi ? kept[r] : r;
     MoveSlot m{-1, 0.f, r - lo};
     if (src != r) {
       const int32_t ps = cache_page(a.c, a.table, b, src, a.status);
@@ -328,7 +329,10 @@ __device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair
     while (leads) {
       const int l = __ffs(leads) - 1;
       leads &= leads - 1;
-      move_block<KIND, D>(a, kv, b, h, pair, __shfl_sync(0xffffffffu, block, l) * bs, slots);
+      const int lo = __shfl_sync(0xffffffffu, block, l) * bs;
+      const int r = lo + lane;
+      const int src0 = lane < bs && r < a.budget ? a.kept[pair * a.budget + r] : r;
+      move_block<KIND, D>(a, kv, b, h, pair, lo, src0, slots);
     }
     return;
   }
@@ -729,16 +733,17 @@ __global__ void __launch_bounds__(32 * kMoveWarps, 4) cache_move_kernel(const Ev
   const int h = static_cast<int>(pair % a.c.Hkv), b = static_cast<int>(pair / a.c.Hkv);
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const int m = a.counts[pair];
-  if (m == 0) return;
   if (!cache_8bit(KIND) || !a.by_block) {
     if (chunk * move_entries(KIND) < m) move_entries_of<KIND, D>(a, pair, b, h, chunk, kv, m, slots);
     return;
   }
   const int lo = chunk * a.c.scale_block;
   const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
-  bool moved = false;
-  for (int r = lo + lane; r < hi; r += 32) moved = moved || a.kept[pair * a.budget + r] != r;
-  if (__any_sync(0xffffffffu, moved)) move_block<KIND, D>(a, kv, b, h, pair, lo, slots);
+  const int32_t* kept = a.kept + pair * a.budget;
+  const int src0 = lo + lane < hi ? kept[lo + lane] : lo + lane;  // asked for together with m
+  bool moved = src0 != lo + lane;
+  for (int r = lo + lane + 32; r < hi; r += 32) moved = moved || kept[r] != r;
+  if (m > 0 && __any_sync(0xffffffffu, moved)) move_block<KIND, D>(a, kv, b, h, pair, lo, src0, slots);
 }
 
 struct EvictPlan {

@@ -392,6 +392,30 @@ def test_bad_pages_and_lengths_are_reported_and_harmless():
     assert np.abs(out - ref["out"]).max() < 1e-2
 
 
+def test_table_entries_behind_the_rows_in_use_may_hold_anything():
+    import pa_b200
+
+    rng = np.random.default_rng(14)
+    c = Cache(rng, 2, 2, 64, 16, 8, "e4m3", [40, 17], 200)
+    a = c.arrays("hnd")
+    t = a["block_table"].copy()
+    t[0, 3:], t[1, 2:] = -7, 10 ** 8
+    b = {**a, "block_table": t}
+    q = rng.standard_normal((2, 4, 64)).astype(np.float16)
+    w = rng.random((2, 2, 200)).astype(np.float32)
+    for x, y in zip(pa_b200.cache_decode(q, seq_lens=[40, 17], weights=w, max_seq_len=200, **a),
+                    pa_b200.cache_decode(q, seq_lens=[40, 17], weights=w, max_seq_len=200, **b)):
+        np.testing.assert_array_equal(x, y)
+    x = rng.standard_normal((2, 8, 2, 64)).astype(np.float16)
+    got, want = (pa_b200.cache_append(x, x, seq_lens=[40, 17], **d) for d in (b, a))
+    np.testing.assert_array_equal(got.key_cache, want.key_cache)
+    np.testing.assert_array_equal(got.k_scales, want.k_scales)
+    got = pa_b200.cache_evict(seq_lens=[40, 17], weights=w, budget=11, recent=4, **b)
+    want = pa_b200.cache_evict(seq_lens=[40, 17], weights=w, budget=11, recent=4, **a)
+    np.testing.assert_array_equal(got.key_cache, want.key_cache)
+    np.testing.assert_array_equal(got.kept, want.kept)
+
+
 # ------------------------------------------------------- device pointers (PyTorch tensors)
 
 class OnDevice:
