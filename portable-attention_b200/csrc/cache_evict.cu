@@ -29,6 +29,12 @@
 // pa_cache_append. The block that `budget` cuts holds places below it and
 // possibly sources at or above it: `select` puts its old scales aside, since
 // `move` changes them while other warps read from it.
+//
+// One row over the budget of 2048 in 512 heads (e4m3): 22 us, nearly all latency
+// (10 us of selection in one wave of CTAs, then the move's chain list -> block ->
+// page and scale -> row). 128 heads of up to 8191 fp16 rows to 3001: 44 us for 137
+// MB. 8 heads of 131071 int8 rows to 16384: 61 us for 71 MB, half of it selection
+// on the clusters' 64 SMs, half the moves' look-ups and recoding.
 #include <math.h>
 
 #include "cache.cuh"
