@@ -261,9 +261,10 @@ pa_status pa_decode_kv_fwd(const pa_kv_cache_desc* desc, const void* q, const vo
  *   scales[page * scale_page_stride + h * scale_head_stride + r / scale_block]
  * and an element stands for code * scale. Paged: scale_block divides page_size.
  * 16-bit caches have no scales (pass NULL; the scale_* fields are not read).
- * Per-row arrays (weights, positions) hold one 4-byte element per row of a
- * sequence and kv head, at b * row_seq_stride + h * row_head_stride + row; the
- * row strides are read only where such an array is passed.
+ * Per-row arrays (weights, positions) hold one 4-byte element for each of the
+ * max_seq_len rows of a sequence and kv head, at
+ * b * row_seq_stride + h * row_head_stride + row; the row strides are read only
+ * where such an array is passed.
  *
  * Lengths outside [0, max_seq_len] and block-table entries outside
  * [0, num_pages) are detected on the device and reported by
@@ -271,8 +272,9 @@ pa_status pa_decode_kv_fwd(const pa_kv_cache_desc* desc, const void* q, const vo
  * and pa_cache_decode reads such rows as zeros.
  *
  * All calls are asynchronous on `stream`, allocate nothing when given a
- * workspace, and can be captured into a CUDA graph. Workspaces of calls that
- * may overlap on the GPU must be different.
+ * workspace (16-byte aligned), and can be captured into a CUDA graph; the first
+ * call on a device sets up the library's status word there, so make one before a
+ * capture. Workspaces of calls that may overlap on the GPU must be different.
  */
 typedef struct pa_block_cache_desc {
   pa_kv_cache_desc cache;
@@ -318,7 +320,8 @@ pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new, co
 /*
  * Decode over a block-scaled cache: as pa_decode_kv_fwd (same q, out, lse,
  * grouped heads, empty sequences, rows past the length never used), with the
- * scales above. NULL seq_lens means max_seq_len keys everywhere.
+ * scales above; q and out are 16-byte aligned. NULL seq_lens means max_seq_len
+ * keys everywhere. Table entries behind a sequence's rows may hold anything.
  * `weights` (optional): weights[b][h][j] += the softmax weight of key j, summed
  * over the query heads of kv head h, for every row j of the sequence.
  * Scales of rows in use must be finite; value scales below 2^-120 in magnitude

@@ -326,6 +326,33 @@ def test_evict_of_long_sequences(fmt, B, H, n, budget, page, block):
     c.check_equal(got, "hnd")
 
 
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("layout", ["hnd", "nhd"])
+def test_dense_cache_append_decode_evict(fmt, layout):
+    """No block table: page b is sequence b, and scale blocks need not divide it."""
+    import pa_b200
+
+    rng = np.random.default_rng(41)
+    B, Hq, H, D, page, block, T, budget = 3, 6, 2, 64, 157, 12, 30, 70
+    lens = np.array([100, 0, 127], np.int32)
+    c = Cache(rng, B, H, D, page, block, fmt, lens, page, paged=False)
+    x = rng.standard_normal((2, B, T, H, D)).astype(np.float16)
+    got = pa_b200.cache_append(x[0], x[1], seq_lens=lens, **c.arrays(layout))
+    append_reference(x[0], x[1], c.k, c.v, lens, [T] * B, fmt=fmt, **c.parts())
+    c.check_equal(got, layout)
+    lens = got.seq_lens
+    q = rng.standard_normal((B, Hq, D)).astype(np.float16)
+    before = rng.random((B, H, page)).astype(np.float32)
+    out, lse, w = pa_b200.cache_decode(q, seq_lens=lens, weights=before, return_lse=True, **c.arrays(layout))
+    check_decode(decode_reference(q, c.k, c.v, lens, weights=before, **c.parts()), out, lse, w, before)
+    want_w = w.copy()
+    got = pa_b200.cache_evict(seq_lens=lens, weights=w, budget=budget, recent=9, sinks=2, **c.arrays(layout))
+    want_len, kept = evict_reference(c.k, c.v, lens, want_w, budget, recent=9, sinks=2, fmt=fmt, **c.parts())
+    np.testing.assert_array_equal(got.kept, kept)
+    np.testing.assert_array_equal(got.weights, want_w)
+    c.check_equal(got, layout)
+
+
 def test_a_budgeted_serving_loop():
     """Prompt, then tokens: append, decode with weights, evict when over budget, against the oracle
     (which takes the device's own weights, so a close call in the choice cannot split the two)."""
@@ -668,6 +695,63 @@ def test_offsets_past_32_bits():
     np.testing.assert_array_equal(sc[~np.isnan(s)], s[~np.isnan(s)].astype(np.float32))
     ref = decode_reference(q.cpu().numpy(), c, c, [T, T], ks=s, vs=s, table=tab, block=block, weights=w0)
     check_decode(ref, out.cpu().numpy(), lse.cpu().numpy(), w.cpu().numpy(), w0)
+
+
+@pytest.mark.parametrize("H,n,budget", [(2, 9004, 4000), (80, 301, 120)])
+def test_evict_writes_positions_without_being_given_any(H, n, budget):
+    """positions_out holds the rows themselves; weights at an odd address, results apart from the inputs,
+    what is behind the new length left as it was (one head in a cluster, many in one CTA each)."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(n)
+    c = Cache(rng, 1, H, 64, 64, 64, None, [n], n)
+    d = OnDevice(c, "hnd")
+    w = torch.rand(H * n + 1, device="cuda")[1:]
+    w_out, p_out = torch.full((H, n), -2.0, device="cuda"), torch.full((H, n), -3, dtype=torch.int32, device="cuda")
+    lens2, kept = torch.empty_like(d.lens), torch.empty((H, budget), dtype=torch.int32, device="cuda")
+    want_w = w.cpu().numpy().reshape(1, H, n).copy()
+    pa_b200.cache_evict_device(d.desc(H, n), d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(), w.data_ptr(), budget,
+                               lens2.data_ptr(), kept.data_ptr(), recent=5, weights_out_ptr=w_out.data_ptr(),
+                               positions_out_ptr=p_out.data_ptr(), **d.kw())
+    torch.cuda.synchronize()
+    pa_b200.sync_device_status()
+    _, want = evict_reference(c.k, c.v, [n], want_w, budget, recent=5, table=c.table)
+    np.testing.assert_array_equal(kept.cpu().numpy(), want[0])
+    np.testing.assert_array_equal(p_out[:, :budget].cpu().numpy(), want[0])
+    np.testing.assert_array_equal(w_out[:, :budget].cpu().numpy(), want_w[0, :, :budget])
+    assert (w_out[:, budget:] == -2).all() and (p_out[:, budget:] == -3).all()
+    d.check_equal()
+
+
+def test_two_streams_at_once_without_workspaces_or_lengths():
+    """Scratch from the pool; NULL lengths mean full sequences. Each stream's calls repeat bit for bit."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(51)
+    rows, sides = 1024, []
+    for fmt in ("e4m3", None):
+        c = Cache(rng, 3, 2, 128, 32, 32, fmt, [rows] * 3, rows)
+        d = OnDevice(c, "nhd")
+        q = torch.randn((3, 8, 128), device="cuda").half()
+        out, w = torch.empty_like(q), torch.zeros((3, 2, rows), device="cuda")
+        sides.append((c, d, d.desc(8, rows), q, out, w, torch.cuda.Stream()))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for c, d, desc, q, out, w, s in sides:
+            pa_b200.cache_decode_device(desc, q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), out.data_ptr(), weights_ptr=w.data_ptr(),
+                                        stream=On(s), **d.kw())
+    torch.cuda.synchronize()
+    pa_b200.sync_device_status()
+    for c, d, desc, q, out, w, s in sides:
+        ref = decode_reference(q.cpu().numpy(), c.k, c.v, [rows] * 3, weights=np.zeros((3, 2, rows)), **c.parts())
+        tol = U["f16"] * np.abs(ref["out"]) + (2.0 ** -11 + 2.0 ** -16) * ref["pv"] + 2.0 ** -25
+        assert (np.abs(out.double().cpu().numpy() - ref["out"]) <= tol).all()
+        # Twenty equal additions: each within the single call's bound, and half a step of the sum each time.
+        dl = (2.0 ** -18 * ref["mag"] + 2.0 ** -20 * (1 + np.abs(ref["lse"]))).reshape(3, 2, 4).max(-1)[..., None]
+        want = 20 * ref["weights"]
+        assert (np.abs(w.cpu().numpy() - want) <= want * (2 * dl + 2.0 ** -18 + 20 * 2.0 ** -24)).all()
 
 
 def test_calls_on_another_device():
