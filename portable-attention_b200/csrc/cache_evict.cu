@@ -46,6 +46,7 @@ constexpr int kBins = 2048;     // digits of 11 bits (the last: 10)
 constexpr int kScanThreads = 256;
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxCluster = 8;  // portable cluster size
+constexpr int kFewRows = 8;     // rows to evict that are picked one by one
 
 struct EvictArgs {
   CacheView c;
@@ -513,6 +514,77 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   };
 
   // ------------------------------------------------ threshold: radix selection
+  // What `move` needs apart from the lists, by one thread or two.
+  auto put_aside = [&](int moves) {
+    if (rank == 0 && tid == 0) a.counts[pair] = moves;
+    if (cache_8bit(a.c.kind) && rank == 0 && tid < 2 && n % a.c.scale_block) {
+      const int32_t page = cache_page(a.c, a.table, b, n, a.status);
+      a.cut_scale[pair * 2 + tid] = page < 0 ? 0.f : a.scales[tid][cache_scale(a.c, page, h, cache_at(a.c, n))];
+    }
+  };
+
+  // ------------------------------------------- a few rows: one minimum at a time
+  // The rows that go are the smallest keys, the highest row among equals; a budget
+  // that is kept up every step evicts one. No digits are counted and no ranks
+  // summed: the holes are the evicted rows below the budget, the sources the rows
+  // behind it that were not evicted.
+  if (C == 1 && rounds == 1 && len - n <= kFewRows) {
+    rank_keys();
+    copy_rows();
+    const int warp = tid >> 5, warps = T >> 5, out = len - n;
+    for (int i = 0; i < out; ++i) {
+      uint32_t key = 0xffffffffu;
+      int row = -1;
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k)
+        if ((live >> k & 1u) && keys[k] <= key) {  // a thread's rows ascend
+          key = keys[k];
+          row = static_cast<int>(row_of(k));
+        }
+      const uint32_t wk = __reduce_min_sync(0xffffffffu, key);
+      const int wr = __reduce_max_sync(0xffffffffu, key == wk ? row : -1);
+      if (lane == 0) {
+        sh.warp_sum[0][warp] = static_cast<int>(wk);
+        sh.warp_sum[1][warp] = wr;
+      }
+      __syncthreads();
+      const int r = lane < warps ? sh.warp_sum[1][lane] : -1;
+      const uint32_t v = r >= 0 ? static_cast<uint32_t>(sh.warp_sum[0][lane]) : 0xffffffffu;
+      const uint32_t least = __reduce_min_sync(0xffffffffu, v);
+      const int gone = __reduce_max_sync(0xffffffffu, v == least ? r : -1);
+#pragma unroll
+      for (int k = 0; k < kKeys; ++k)
+        if (row_of(k) == gone) live &= ~(1u << k);
+      if (tid == 0) sh.own[i] = gone;
+      __syncthreads();
+    }
+    if (tid < 32) {
+      const int e = lane < out ? sh.own[lane] : 0x7fffffff;
+      int before = 0, kept_before = 0;
+      bool evicted = false;
+      for (int i = 0; i < out; ++i) {
+        const int x = sh.own[i];
+        before += x < e;
+        kept_before += x >= n && x < n + lane;
+        evicted = evicted || x == n + lane;
+      }
+      if (e < n) sh.hist[0][before] = e;
+      if (lane < out && !evicted) sh.hist[1][lane - kept_before] = n + lane;
+      const int moves = __popc(__ballot_sync(0xffffffffu, e < n));
+      __syncwarp();
+      if (lane < moves) {
+        const int d = sh.hist[0][lane], q = sh.hist[1][lane];
+        holes[lane] = d;
+        sources[lane] = q;
+        kept[d] = q;
+        if (w_out) w_out[d] = w[q];
+        if (p_out) p_out[d] = pos ? pos[q] : q;
+      }
+      put_aside(moves);
+    }
+    return;
+  }
+
   // A cluster's CTAs add into each other's arrays, so all are cleared up front.
   for (int i = tid; i < (C > 1 ? 4 : 1) * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
   if (C > 1) fetch(row0, row_end);
@@ -716,11 +788,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
       }
     }
   }
-  if (rank == 0 && tid == 0) a.counts[pair] = hole_all;
-  if (cache_8bit(a.c.kind) && rank == 0 && tid < 2 && n % a.c.scale_block) {
-    const int32_t page = cache_page(a.c, a.table, b, n, a.status);
-    a.cut_scale[pair * 2 + tid] = page < 0 ? 0.f : a.scales[tid][cache_scale(a.c, page, h, cache_at(a.c, n))];
-  }
+  put_aside(hole_all);
 }
 
 // The rows of 8-bit caches where moves can be as many as blocks: a warp has one

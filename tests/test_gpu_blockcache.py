@@ -304,6 +304,33 @@ def test_evict_without_positions_and_with_equal_weights():
     assert list(got.seq_lens) == [40, 40]
 
 
+@pytest.mark.parametrize("over", [1, 2, 7, 8, 9])
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_evict_of_a_few_rows(fmt, over):
+    """A budget kept up step by step: few rows over it, ties, protected rows among the smallest."""
+    import pa_b200
+
+    rng = np.random.default_rng(over)
+    B, H, budget = 4, 3, 261
+    lens = np.array([budget + over, budget + 1, budget, budget + over], np.int32)
+    c = Cache(rng, B, H, 64, 16, 8, fmt, lens, budget + over)
+    w = np.round(rng.exponential(size=(B, H, budget + over)) * 30).astype(np.float32) / 30
+    w[0, 0] = 1.0                                       # all equal: the last unprotected rows go
+    w[1, 1, 5] = np.nan
+    w[3, :, budget:] = 50.0                             # every row behind the budget stays
+    w[3, 2, 250:258] = w[3, 2, 3]
+    for recent, sinks in ((0, 0), (20, 4), (255, 6)):
+        d = Cache.__new__(Cache)
+        d.__dict__.update({k: v.copy() if isinstance(v, np.ndarray) else v for k, v in c.__dict__.items()})
+        got = pa_b200.cache_evict(seq_lens=lens, weights=w, budget=budget, recent=recent, sinks=sinks, **d.arrays("nhd"))
+        want_w = w.copy()
+        want_len, kept = evict_reference(d.k, d.v, lens, want_w, budget, recent=recent, sinks=sinks, fmt=fmt, **d.parts())
+        np.testing.assert_array_equal(got.kept, kept)
+        np.testing.assert_array_equal(got.weights, want_w)
+        np.testing.assert_array_equal(got.seq_lens, want_len)
+        d.check_equal(got, "nhd")
+
+
 @pytest.mark.parametrize("fmt,B,H,n,budget,page,block", [
     ("int8", 1, 1, 140001, 20003, 64, 64),     # a cluster whose threads hold their rows in two rounds
     (None, 40, 2, 17001, 16990, 1024, 1024),   # one CTA a head, three rounds
