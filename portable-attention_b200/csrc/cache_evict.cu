@@ -10,7 +10,8 @@
 // move are touched (an order-keeping compaction would move every row behind the
 // first hole).
 //
-// Two launches, the second started while the first ends. `select`: a (sequence,
+// Two launches, the second started while the first ends (one where few rows can
+// go). `select`: a (sequence,
 // kv head) is one CTA, or a cluster of up to eight where there are few of them.
 // Each thread holds eight or sixteen rows' keys in registers, four neighbours at a
 // time so that a warp's reads are whole lines (longer shares are read again in
@@ -30,9 +31,9 @@
 // possibly sources at or above it: `select` puts its old scales aside, since
 // `move` changes them while other warps read from it.
 //
-// One row over the budget of 2048 in 512 heads (e4m3): 22 us, nearly all latency
-// (10 us of selection in one wave of CTAs, then the move's chain list -> block ->
-// page and scale -> row). 128 heads of up to 8191 fp16 rows to 3001: 44 us for 137
+// One row over the budget of 2048 in 512 heads (e4m3): 14.4 us, nearly all latency
+// (keys, the minimum, then the move's chain list -> block -> page and scale -> row;
+// 22 us when digits were counted and rows moved by a second launch). 128 heads of up to 8191 fp16 rows to 3001: 44 us for 137
 // MB. 8 heads of 131071 int8 rows to 16384: 61 us for 71 MB, half of it selection
 // on the clusters' 64 SMs, half the moves' look-ups and recoding.
 #include <math.h>
@@ -380,7 +381,10 @@ __device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair
 
 // kThreads and kCtas bound the registers: 1024 threads, or four CTAs of 256 to 320
 // for many short sequences, so that 512 of them run at once.
-template <int kKeys, int kThreads, int kCtas>
+// kMoveKind >= 0: at most kFewRows rows go, and the CTA carries the rows over too
+// (the rest of the kernel is then not reached).
+#pragma nv_diag_suppress 128
+template <int kKeys, int kThreads, int kCtas, int kMoveKind, int kMoveD>
 __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const EvictArgs a) {
   extern __shared__ __align__(16) uint8_t smem_raw[];
   EvictShared& sh = *reinterpret_cast<EvictShared*>(smem_raw);
@@ -581,9 +585,18 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
         if (p_out) p_out[d] = pos ? pos[q] : q;
       }
       put_aside(moves);
+      if (lane == 0) sh.left = moves;
+    }
+    if constexpr (kMoveKind >= 0) {
+      __syncthreads();
+      MoveSlot* const slots = reinterpret_cast<MoveSlot*>(&sh.hist[2][0]) + warp * 32;
+      constexpr int kSides = cache_8bit(kMoveKind) ? 2 : 1;
+      if (warp < kSides && sh.left > 0)
+        move_entries_of<kMoveKind, kMoveD>(a, pair, b, h, 0, warp, sh.left, slots);
     }
     return;
   }
+  if (kMoveKind >= 0) return;
 
   // A cluster's CTAs add into each other's arrays, so all are cleared up front.
   for (int i = tid; i < (C > 1 ? 4 : 1) * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
@@ -840,9 +853,9 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
 
 // A CTA per (sequence, kv head), or a cluster of 2, 4 or 8 while each CTA then has
 // an SM and 2048 rows (128 heads of 8191 rows: 44.0 us alone, 49.0 in pairs); threads for eight rows each, sixteen
-// where 1024 threads of eight would need a second round. (Carrying few moves over
-// in the same CTA instead of a second launch measured the same, 22.5 us for one
-// row of 2049 in 512 heads.)
+// where 1024 threads of eight would need a second round. Where no sequence can be
+// more than kFewRows over the budget, the CTA carries the rows over itself (one row
+// of 2049 in 512 heads: 14.4 us, with a second launch 16.9).
 template <int KIND, int D>
 pa_status launch_evict(EvictArgs a, cudaStream_t st) {
   const int64_t pairs = static_cast<int64_t>(a.c.B) * a.c.Hkv;
@@ -864,9 +877,13 @@ pa_status launch_evict(EvictArgs a, cudaStream_t st) {
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = cluster > 1 ? 1 : 0;
-  PA_CUDA(cudaLaunchKernelEx(&cfg, keys == 16       ? cache_select_kernel<16, kMaxThreads, 1>
-                                   : threads <= 320 ? cache_select_kernel<8, 320, 4>
-                                                    : cache_select_kernel<8, kMaxThreads, 1>, a));
+  if (a.c.max_len - a.budget <= kFewRows && a.list > 0 && cluster == 1 && share <= threads * 8 && threads <= 320) {
+    PA_CUDA(cudaLaunchKernelEx(&cfg, cache_select_kernel<8, 320, 4, KIND, D>, a));
+    return PA_OK;
+  }
+  PA_CUDA(cudaLaunchKernelEx(&cfg, keys == 16       ? cache_select_kernel<16, kMaxThreads, 1, -1, 0>
+                                   : threads <= 320 ? cache_select_kernel<8, 320, 4, -1, 0>
+                                                    : cache_select_kernel<8, kMaxThreads, 1, -1, 0>, a));
   if (a.list == 0) return PA_OK;
   int32_t chunks = (a.list + move_entries(KIND) - 1) / move_entries(KIND);
   if (cache_8bit(KIND)) {
