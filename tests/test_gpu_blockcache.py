@@ -781,6 +781,39 @@ def test_two_streams_at_once_without_workspaces_or_lengths():
         assert (np.abs(w.cpu().numpy() - want) <= want * (2 * dl + 2.0 ** -18 + 20 * 2.0 ** -24)).all()
 
 
+def test_calls_with_workspaces_allocate_nothing():
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(61)
+    c = Cache(rng, 2, 2, 64, 16, 16, "int8", [4000, 9], 4200)
+    d = OnDevice(c, "hnd")
+    desc = d.desc(4, 4200)
+    q, x = torch.randn((2, 4, 64), device="cuda").half(), torch.randn((2, 2, 8, 2, 64), device="cuda").half()
+    out, w = torch.empty_like(q), torch.zeros((2, 2, 4200), device="cuda")
+    lens2, lens3 = torch.empty_like(d.lens), torch.empty_like(d.lens)
+    kept = torch.empty((2, 2, 3000), dtype=torch.int32, device="cuda")
+    n1, n2 = pa_b200.cache_decode_workspace_size(desc, True, True), pa_b200.cache_evict_workspace_size(desc, True, 3000)
+    ws = torch.empty((max(n1, n2),), dtype=torch.uint8, device="cuda")
+
+    def step():
+        pa_b200.cache_append_device(desc, x[0].data_ptr(), x[1].data_ptr(), 8, d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(),
+                                    weights_ptr=w.data_ptr(), seq_lens_out_ptr=lens2.data_ptr(), **d.kw())
+        pa_b200.cache_decode_device(desc, q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), out.data_ptr(), seq_lens_ptr=lens2.data_ptr(),
+                                    weights_ptr=w.data_ptr(), workspace=(ws.data_ptr(), n1), **d.kw())
+        pa_b200.cache_evict_device(desc, d.k.data_ptr(), d.v.data_ptr(), lens2.data_ptr(), w.data_ptr(), 3000, lens3.data_ptr(),
+                                   kept.data_ptr(), weights_out_ptr=w.data_ptr(), workspace=(ws.data_ptr(), n2), **d.kw())
+
+    step()
+    torch.cuda.synchronize()
+    free = torch.cuda.mem_get_info()[0]
+    for _ in range(10):
+        step()
+    torch.cuda.synchronize()
+    assert torch.cuda.mem_get_info()[0] == free
+    assert lens3.tolist() == [3000, 17]
+
+
 def test_calls_on_another_device():
     import pa_b200
 
