@@ -294,9 +294,12 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
   // ----------------------------------------------------------- Q fragments
   // Thread (g, c) = (lane / 4, lane % 4) holds head rows g and g + 8. For 8-bit
   // caches the head-dim order is permuted per thread (a dot product does not see
-  // it), and a bf16 query is scaled by a power of two into fp16's range.
+  // it), and a bf16 query becomes fp16 after a power of two of its own head that
+  // puts the head's largest element into [2^14, 2^15): heads of one group may differ
+  // in magnitude by any factor, and elements down to 2^-28 of their head's largest
+  // keep all their bits.
   const int g = lane >> 2, c = lane & 3;
-  float sl2 = a.scale_log2;
+  float sl2 = a.scale_log2, sl2_hi = a.scale_log2;  // of heads g and g + 8
   uint32_t qa[KS][2], qh[KS][2];
   {
     const uint32_t* qw = static_cast<const uint32_t*>(a.q) + q0 * (D / 2);
@@ -312,33 +315,32 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
         qh[s][w] = kTwo ? frag(g + 8, s, w) : 0u;
       }
     if (QBF16 && kF8) {
-      float mx = 0.f;
+      // One head, held by the four lanes of equal g; returns scale_log2 over its factor.
+      auto to_f16 = [&](uint32_t (&f)[KS][2]) -> float {
+        float mx = 0.f;
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const float2 f = cache_unpack<true>(qa[s][w]), f2 = cache_unpack<true>(qh[s][w]);
-          mx = cache_amax(cache_amax(cache_amax(cache_amax(mx, f.x), f.y), f2.x), f2.y);
-        }
-      mx = warp_max(mx);
-      float qs = 1.f;
-      if (mx > 0.f) {
+          for (int w = 0; w < 2; ++w) {
+            const float2 x = cache_unpack<true>(f[s][w]);
+            mx = cache_amax(cache_amax(mx, x.x), x.y);
+          }
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
         int e = static_cast<int>(__float_as_uint(mx) >> 23) - 127;  // floor(log2(mx)) for normal values
         e = e < -100 ? -100 : e;
-        qs = __int_as_float((127 + 14 - e) << 23);  // mx * qs in [2^14, 2^15)
-        sl2 = a.scale_log2 * __int_as_float((127 - 14 + e) << 23);
-      }
+        const float qs = __int_as_float((127 + 14 - e) << 23);
 #pragma unroll
-      for (int s = 0; s < KS; ++s)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int w = 0; w < 2; ++w) {
-          const float2 f = cache_unpack<true>(qa[s][w]);
-          qa[s][w] = pack_pair<false>(f.x * qs, f.y * qs);
-          if (kTwo) {
-            const float2 f2 = cache_unpack<true>(qh[s][w]);
-            qh[s][w] = pack_pair<false>(f2.x * qs, f2.y * qs);
+          for (int w = 0; w < 2; ++w) {
+            const float2 x = cache_unpack<true>(f[s][w]);
+            f[s][w] = pack_pair<false>(x.x * qs, x.y * qs);
           }
-        }
+        return a.scale_log2 * __int_as_float((127 - 14 + e) << 23);
+      };
+      sl2 = to_f16(qa);
+      if (kTwo) sl2_hi = to_f16(qh);
     }
   }
 
@@ -416,13 +418,14 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
         const float4 fk = *reinterpret_cast<const float4*>(sc + 8 * nt + 4 * c);
         const float4 fv = *reinterpret_cast<const float4*>(sc + TK + 8 * nt + 4 * c);
         const float k4[4] = {fk.x * sl2, fk.y * sl2, fk.z * sl2, fk.w * sl2};
+        const float k4_hi[4] = {fk.x * sl2_hi, fk.y * sl2_hi, fk.z * sl2_hi, fk.w * sl2_hi};
         const float v4[4] = {fv.x, fv.y, fv.z, fv.w};
 #pragma unroll
         for (int u = 0; u < 2; ++u)
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             sacc[nt + u][e] *= k4[2 * u + e];
-            if (kTwo) sacc[nt + u][2 + e] *= k4[2 * u + e];
+            if (kTwo) sacc[nt + u][2 + e] *= (QBF16 ? k4_hi : k4)[2 * u + e];
             vw[nt + u][e] = v4[2 * u + e];
             vmax = fmaxf(vmax, fabsf(v4[2 * u + e]));
           }
