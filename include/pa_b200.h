@@ -324,9 +324,8 @@ pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new, co
  * keys everywhere. Table entries behind a sequence's rows may hold anything.
  * `weights` (optional): weights[b][h][j] += the softmax weight of key j, summed
  * over the query heads of kv head h, for every row j of the sequence.
- * Scales of rows in use must be finite; value scales below 2^-120 in magnitude
- * count as 0. The cache may span 2^32 times the largest power of two that divides
- * its strides in bytes (16 at least).
+ * Scales of rows in use must be finite. The cache may span 2^32 times the
+ * largest power of two that divides its strides in bytes (16 at least).
  */
 pa_status pa_cache_decode_workspace_size(const pa_block_cache_desc* desc, int32_t paged,
                                          int32_t with_weights, size_t* bytes);

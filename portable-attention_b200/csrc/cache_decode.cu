@@ -19,11 +19,13 @@
 // Per tile, on tensor cores (m16n8k16, fp32 accumulators), operand layout as in
 // decode.cu: S = Q K^T with the G query heads as rows, then O^T = V^T P^T with P
 // straight from the S accumulators. P is rounded to fp16 relative to the tile:
-//   p'_j = 2^(s_j - m_tile) * vs_j / max|vs| * 2^15,
-// and the tile's O^T joins the running one in fp32 with the factor
-// 2^(m_tile - m_run) * max|vs| * 2^-15. A probability down to 2^-29 of its tile's
-// largest keeps all 11 bits, whatever the other tiles hold: a first token that
-// takes nearly all the weight, as trained models have, costs the others nothing.
+//   p'_j = 2^(s_j - m_tile) * vs_j / 2^e * 2^14,  2^e <= max|vs| < 2^(e+1)
+// (2^15 where there are no scales), and the tile's O^T joins the running one in
+// fp32 with the factor 2^(m_tile - m_run) * 2^(e-14). A power of two is exact at both
+// ends of fp32's range, where a reciprocal of max|vs| is not. A probability down to
+// 2^-28 of its tile's largest keeps all 11 bits, whatever the other tiles hold: a
+// first token that takes nearly all the weight, as trained models have, costs the
+// others nothing.
 // bf16 caches need bf16 products; there p' has no factor (bf16 has the range, and
 // values near its end must not overflow the sums) and goes in as two bf16 terms.
 //
@@ -53,7 +55,6 @@ constexpr float kLn2 = 0.6931471805599453f;
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
 constexpr int kMaxSplit = 512;
-constexpr float kMinScale = 7.52316385e-37f;  // 2^-120
 
 template <int KIND, int D, int HT>
 struct DecCfg {
@@ -408,7 +409,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
 
     // ---- softmax of the tile: keys key_of(nt, e) of heads g (columns 0-1), g + 8 (2-3)
     auto key_of = [&](int nt, int e) { return kF8 ? 16 * (nt >> 1) + 4 * c + 2 * (nt & 1) + e : 8 * nt + 2 * c + e; };
-    float vw[NT][2];      // value scale over the tile's largest, times kPScale
+    float vw[NT][2];      // value scale over the power of two of the tile's largest, times 2^14
     float vtile = 1.f / kPScale;
     if (kF8) {
       const float* sc = reinterpret_cast<const float*>(kt + C::kScaleOff);
@@ -432,8 +433,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
       }
       vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 1));
       vmax = fmaxf(vmax, __shfl_xor_sync(0xffffffffu, vmax, 2));
-      const float r = vmax >= kMinScale ? __fdividef(kPScale, vmax) : 0.f;
-      vtile = vmax * (1.f / kPScale);
+      // Scales below 2^-112 stay as far below the factor as they are.
+      const uint32_t e = max(__float_as_uint(vmax) >> 23, 15u);
+      const float r = __uint_as_float((2u * 127u + 14u - e) << 23);
+      vtile = __uint_as_float((e - 14u) << 23);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         vw[nt][0] *= r;

@@ -52,3 +52,33 @@ def test_bf16_query_heads_of_one_group_far_apart_in_magnitude(fmt, D, Hq):
     ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, lens, weights=w, **c.parts())
     check_decode({k: v[:, 1::2] if k != "weights" else v for k, v in ref.items()}, out[:, 1::2], lse[:, 1::2], u=U["bf16"])
     assert np.isfinite(got_w).all()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+@pytest.mark.parametrize("exp", [127, 100, -112, -118, -125])
+def test_value_scales_at_the_ends_of_fp32(fmt, exp):
+    """Scales of 1 to 1.9 times 2^exp: bf16 holds the results, which are below a code times its scale.
+
+    From 2^-117 down a result may be a bf16 subnormal: half a step of those is 2^-134, and fp32
+    sums lose at most 2^-149 a tile (of four), taken relative to 256 rows."""
+    import torch
+
+    rng = np.random.default_rng(exp + 200)
+    rows, lens = 200, [200, 5]
+    c = Cache(rng, 2, 2, 64, 16, 8, fmt, lens, rows)
+    live = ~np.isnan(c.vs)
+    c.vs[live] = (np.float32(1 + 0.9 * rng.random(live.sum())) * np.float32(2.0) ** np.float32(exp)).astype(np.float64)
+    if exp > 0:                                # codes whose product with the scale is finite in bf16
+        c.v = np.clip(c.v, -1, 1)
+        if exp == 127:
+            c.v[:] = np.where(np.isnan(c.v), c.v, 0.0)
+            for b in range(2):                 # one row of codes 1, the others 0
+                c.v[c.table[b, 0], :, 3] = 1.0
+    d = OnDevice(c, "hnd")
+    q = torch.from_numpy(rng.standard_normal((2, 4, 64))).to("cuda", torch.bfloat16)
+    out, lse, _ = decode(d, q, rows)
+    ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, lens, **c.parts())
+    assert (np.abs(ref["out"]).max((1, 2)) > 2.0 ** (exp - 12)).all()
+    tol = U["bf16"] * np.abs(ref["out"]) + (2.0 ** -11 + 2.0 ** -16) * ref["pv"] + 2.0 ** -134 + 2.0 ** -139
+    assert np.isfinite(out).all()
+    assert (np.abs(out - ref["out"]) <= tol).all(), float((np.abs(out - ref["out"]) / tol).max())
