@@ -26,8 +26,11 @@
 // 2^-28 of its tile's largest keeps all 11 bits, whatever the other tiles hold: a
 // first token that takes nearly all the weight, as trained models have, costs the
 // others nothing.
-// bf16 caches need bf16 products; there p' has no factor (bf16 has the range, and
-// values near its end must not overflow the sums) and goes in as two bf16 terms.
+// bf16 caches need bf16 products; there p' has the factor 2^-5 (bf16 has the range,
+// and a tile's 32 rows near its end must not overflow) and goes in as two bf16 terms.
+// The running O^T carries a factor 2^-k, 2^k >= max_len: sums over all rows stay below
+// the largest value that a row has, so an output that is finite comes out finite.
+// What that costs are the last k bits of outputs near fp32's smallest.
 //
 // Splits leave (max, sum, accumulator) in the workspace and a second launch joins
 // them by log-sum-exp; a single split without weights writes its output itself.
@@ -105,6 +108,7 @@ struct DecodeArgs {
   uint32_t u_page, u_head, u_key;  // the strides in units
   uint32_t u_scale_page;
   float scale_log2;
+  float acc_scale;   // 2^-k of the running O^T
 };
 
 __device__ __forceinline__ int seq_len(const DecodeArgs& a, int b, bool report) {
@@ -193,7 +197,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
   constexpr bool kF8 = cache_8bit(KIND);
   constexpr bool kMmaBf16 = KIND == kCacheBF16;
   constexpr bool kTwo = HT == 16;
-  constexpr float kPScale = kMmaBf16 ? 1.f : 32768.f;
+  constexpr float kPScale = kMmaBf16 ? 0.03125f : 32768.f;
   constexpr int TK = C::kTK;
   constexpr int KS = D / 16;   // k-steps of Q K^T
   constexpr int MT = D / 16;   // m-tiles of V^T P^T
@@ -410,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
     // ---- softmax of the tile: keys key_of(nt, e) of heads g (columns 0-1), g + 8 (2-3)
     auto key_of = [&](int nt, int e) { return kF8 ? 16 * (nt >> 1) + 4 * c + 2 * (nt & 1) + e : 8 * nt + 2 * c + e; };
     float vw[NT][2];      // value scale over the power of two of the tile's largest, times 2^14
-    float vtile = 1.f / kPScale;
+    float vtile = a.acc_scale / kPScale;
     if (kF8) {
       const float* sc = reinterpret_cast<const float*>(kt + C::kScaleOff);
       float vmax = 0.f;
@@ -436,7 +440,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
       // Scales below 2^-112 stay as far below the factor as they are.
       const uint32_t e = max(__float_as_uint(vmax) >> 23, 15u);
       const float r = __uint_as_float((2u * 127u + 14u - e) << 23);
-      vtile = __uint_as_float((e - 14u) << 23);
+      vtile = __uint_as_float((e - 14u) << 23) * a.acc_scale;
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         vw[nt][0] *= r;
@@ -617,7 +621,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
       L = fmaf(f, lw[w * 16 + head], L);
     }
     if (a.direct) {
-      store_out<QBF16>(a, q0 * D + i, L == 0.f ? 0.f : acc / L);
+      store_out<QBF16>(a, q0 * D + i, L == 0.f ? 0.f : acc / (L * a.acc_scale));
       if (a.lse && d == 0) a.lse[q0 + head] = lse_of(M, L) * kLn2;
       continue;
     }
@@ -685,7 +689,7 @@ __global__ void __launch_bounds__(kFinThreads) cache_finish_kernel(const DecodeA
       const float* ml = a.ws_ml + (q0 + g0 + warp) * ns * 2;
       for (int s = lane; s < ns; s += 32) {
         const float ms = ml[2 * s];
-        fac[warp * kMost + s] = ms == -INFINITY ? 0.f : ex2(ms - z);
+        fac[warp * kMost + s] = ms == -INFINITY ? 0.f : ex2(ms - z) / a.acc_scale;
       }
       if (lane == 0 && a.lse && blockIdx.y * E % D == 0) a.lse[q0 + g0 + warp] = z * kLn2;
     }
@@ -937,6 +941,8 @@ extern "C" pa_status pa_cache_decode(const pa_block_cache_desc* desc, const void
   a.u_head = static_cast<uint32_t>(p.c.head_stride / p.unit);
   a.u_key = static_cast<uint32_t>(p.c.key_stride / p.unit);
   a.scale_log2 = static_cast<float>(desc->cache.scale * 1.4426950408889634);
+  a.acc_scale = 1.f;
+  for (int64_t rows = 1; rows < p.c.max_len; rows *= 2) a.acc_scale *= 0.5f;
   void* own = nullptr;
   if (!workspace) PA_TRY(scratch_alloc(&own, p.bytes, st));
   const size_t slots = p.direct ? 0 : static_cast<size_t>(p.c.B) * p.c.Hq * p.nsplit;

@@ -82,3 +82,41 @@ def test_value_scales_at_the_ends_of_fp32(fmt, exp):
     tol = U["bf16"] * np.abs(ref["out"]) + (2.0 ** -11 + 2.0 ** -16) * ref["pv"] + 2.0 ** -134 + 2.0 ** -139
     assert np.isfinite(out).all()
     assert (np.abs(out - ref["out"]) <= tol).all(), float((np.abs(out - ref["out"]) / tol).max())
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,S,weights", [(64, 33, False), (128, 300, False), (64, 300, True), (128, 70001, False), (64, 20011, True)])
+def test_sums_of_many_values_near_the_end_of_the_range(fmt, D, S, weights):
+    """All keys weigh the same and all values are 1.5 * 2^126: their mean is finite, their sum is not."""
+    import torch
+
+    rng = np.random.default_rng(S)
+    c = Cache(rng, 1, 1, D, 64, 64, fmt, [S], S)
+    for x, s in ((c.k, c.ks), (c.v, c.vs)):
+        x[~np.isnan(x)] = 0.0 if x is c.k else 1.5 * 2.0 ** 126 if fmt is None else 3.0
+        if fmt is not None:
+            s[~np.isnan(s)] = 2.0 ** 125
+    d = OnDevice(c, "hnd", "bf16")
+    q = torch.from_numpy(rng.standard_normal((1, 3, D))).to("cuda", torch.bfloat16)
+    w = np.zeros((1, 1, S), np.float32) if weights else None
+    out, lse, _ = decode(d, q, S, weights=w)
+    assert (np.abs(out / (1.5 * 2.0 ** 126) - 1) <= U["bf16"] + 2.0 ** -11 + 2.0 ** -16).all()
+    np.testing.assert_allclose(lse, np.log(S), rtol=2.0 ** -19)
+
+
+def test_small_bf16_values_keep_their_bits():
+    """Values of about 2^-110 over 70001 rows: far below, 17 bits of the sums' range go to the other end."""
+    import torch
+
+    rng = np.random.default_rng(70)
+    c = Cache(rng, 1, 1, 64, 64, 64, None, [70001], 70001)
+    c.v *= 2.0 ** -110
+    for x in (c.k, c.v):
+        x[:] = torch.from_numpy(x).to(torch.bfloat16).double().numpy()
+    d = OnDevice(c, "hnd", "bf16")
+    q = torch.from_numpy(rng.standard_normal((1, 3, 64))).to("cuda", torch.bfloat16)
+    out, _, _ = decode(d, q, 70001)
+    ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, [70001], **c.parts())
+    # Each of 2188 tiles costs at most 2^-149, taken relative to 2^17 rows: 2^-121.
+    tol = U["bf16"] * np.abs(ref["out"]) + 2.0 ** -11 * ref["pv"] + 2.0 ** -120
+    assert (np.abs(out - ref["out"]) <= tol).all()
