@@ -27,7 +27,8 @@
 // first token that takes nearly all the weight, as trained models have, costs the
 // others nothing.
 // bf16 caches need bf16 products; there p' has the factor 2^-5 (bf16 has the range,
-// and a tile's 32 rows near its end must not overflow) and goes in as two bf16 terms.
+// and a tile's 32 rows near its end must not overflow) and goes in as two bf16 terms,
+// the first cut off and the second never 0, so that an infinite value stays one.
 // The running O^T carries a factor 2^-k, 2^k >= max_len: sums over all rows stay below
 // the largest value that a row has, so an output that is finite comes out finite.
 // What that costs are the last k bits of outputs near fp32's smallest.
@@ -496,10 +497,13 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
         const float p0 = ex2(sacc[nt][e0] - base), p1 = ex2(sacc[nt][e0 + 1] - base);
         psum += p0 + p1;
         const float w0 = p0 * vw[nt][0], w1 = p1 * vw[nt][1];
-        ph[nt >> 1][nt & 1] = pack_pair<kMmaBf16>(w0, w1);
         if (kMmaBf16) {
-          const float2 hi = cache_unpack<true>(ph[nt >> 1][nt & 1]);
-          plo[nt >> 1][nt & 1] = pack_pair<true>(w0 - hi.x, w1 - hi.y);
+          const uint32_t u0 = __float_as_uint(w0), u1 = __float_as_uint(w1);
+          ph[nt >> 1][nt & 1] = byte_perm(u0, u1, 0x7632);  // the upper halves
+          plo[nt >> 1][nt & 1] = pack_pair<true>(__uint_as_float(u0 | 1u) - __uint_as_float(u0 & 0xffff0000u),
+                                                 __uint_as_float(u1 | 1u) - __uint_as_float(u1 & 0xffff0000u));
+        } else {
+          ph[nt >> 1][nt & 1] = pack_pair<false>(w0, w1);
         }
       }
       const float m_new = fmaxf(m_h, mx);

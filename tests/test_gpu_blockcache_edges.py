@@ -120,3 +120,47 @@ def test_small_bf16_values_keep_their_bits():
     # Each of 2188 tiles costs at most 2^-149, taken relative to 2^17 rows: 2^-121.
     tol = U["bf16"] * np.abs(ref["out"]) + 2.0 ** -11 * ref["pv"] + 2.0 ** -120
     assert (np.abs(out - ref["out"]) <= tol).all()
+
+
+@pytest.mark.parametrize("q_dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("fmt", ["e4m3", None])
+@pytest.mark.parametrize("S,weights", [(50, False), (50, True), (5000, True)])
+def test_infinities_and_nan_reach_what_they_belong_to(fmt, q_dtype, S, weights):
+    """One launch and two: a NaN key or query makes its heads NaN, a NaN value its element, an infinite
+    value its element infinite; other heads and sequences are as they would be without."""
+    import torch
+
+    rng = np.random.default_rng(S)
+    t16 = torch.float16 if q_dtype == "f16" else torch.bfloat16
+    B, H, G, D = 5, 2, 3, 64
+    c = Cache(rng, B, H, D, 16, 16, fmt, [S] * B, S)
+    if fmt is None:
+        for x in (c.k, c.v):
+            x[:] = torch.from_numpy(x).to(t16).double().numpy()
+    at = lambda b, r: (c.table[b, r // 16], r % 16)  # noqa: E731
+    p, r = at(0, 41)
+    c.k[p, 0, r, 7] = np.nan                     # sequence 0, kv head 0
+    p, r = at(1, 17)
+    c.v[p, 1, r, 9] = np.nan                     # sequence 1, kv head 1, element 9
+    if fmt is None:
+        for n, (b, row, x) in enumerate([(2, 3, np.inf), (2, 40, -np.inf)]):
+            p, r = at(b, row)
+            c.v[p, n, r, 5 + n] = x              # sequence 2: element 5 of kv head 0, 6 of kv head 1
+        p, r = at(4, 20)
+        c.k[p, 1, r, 0] = np.inf                 # sequence 4, kv head 1: a score of plus or minus infinity
+    d = OnDevice(c, "hnd", q_dtype)
+    q = torch.from_numpy(rng.standard_normal((B, H * G, D))).to("cuda", t16)
+    q[3, 1, 3] = float("nan")                    # sequence 3, head 1
+    q[4, H * G - 1, 0] = 2.0                     # an infinite score: that head is NaN
+    q[4, H * G - 2, 0] = -2.0                    # minus infinity: a key without weight
+    w = rng.random((B, H, S)).astype(np.float32) if weights else None
+    out, lse, got_w = decode(d, q, S, q_dtype, weights=w)
+    with np.errstate(all="ignore"):
+        ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, [S] * B, weights=w, **c.parts())
+    assert (ref["lse"][0] != ref["lse"][0]).tolist() == [True] * G + [False] * G
+    for got, want in ((out, ref["out"]), (lse, ref["lse"])) + (((got_w, ref["weights"]),) if weights else ()):
+        for same in (np.isnan, np.isposinf, np.isneginf):
+            np.testing.assert_array_equal(same(got), same(want))
+    ok = np.isfinite(ref["out"])
+    tol = U[q_dtype] * np.abs(ref["out"]) + (2.0 ** -11 + 2.0 ** -16) * ref["pv"] + 2.0 ** -25
+    assert (np.abs(out[ok] - ref["out"][ok]) <= tol[ok]).all()
