@@ -18,20 +18,31 @@
 //
 // Per tile, on tensor cores (m16n8k16, fp32 accumulators), operand layout as in
 // decode.cu: S = Q K^T with the G query heads as rows, then O^T = V^T P^T with P
-// straight from the S accumulators. P is rounded to fp16 relative to the tile:
+// straight from the S accumulators, taken relative to the tile:
 //   p'_j = 2^(s_j - m_tile) * vs_j / 2^e * 2^14,  2^e <= max|vs| < 2^(e+1)
 // (2^15 where there are no scales), and the tile's O^T joins the running one in
 // fp32 with the factor 2^(m_tile - m_run) * 2^(e-14). A power of two is exact at both
-// ends of fp32's range, where a reciprocal of max|vs| is not. A probability down to
-// 2^-28 of its tile's largest keeps all 11 bits, whatever the other tiles hold: a
-// first token that takes nearly all the weight, as trained models have, costs the
-// others nothing.
-// bf16 caches need bf16 products; there p' has the factor 2^-5 (bf16 has the range,
-// and a tile's 32 rows near its end must not overflow) and goes in as two bf16 terms,
-// the first cut off and the second never 0, so that an infinite value stays one.
-// The running O^T carries a factor 2^-k, 2^k >= max_len: sums over all rows stay below
-// the largest value that a row has, so an output that is finite comes out finite.
-// What that costs are the last k bits of outputs near fp32's smallest.
+// ends of fp32's range, where a reciprocal of max|vs| is not.
+//
+// p' goes in as two 16-bit terms, its leading bits cut off and what they leave: 20
+// bits in fp16 while p is above 2^-18 of its tile's largest, then an absolute 2^-39 of
+// that, whatever the other tiles hold (a first token that takes nearly all the
+// weight, as trained models have, costs the others nothing); 14 bits for bf16 caches,
+// which need bf16 products. With up to four heads the second terms are columns 4 to
+// 7 of P^T, which would be empty: rows 4 to 7 of Q repeat the heads, the sums of both
+// columns meet in the merge, and little is paid (64 x 8 x 32768 e4m3: 632 us with one
+// term, 638 with two; the same time in fp16). Larger groups take products of their
+// own (16 x 8 x 32768 e4m3: 8 heads 183 and 196 us, 16 heads 235 and 274; 32 x 8 x
+// 4097 fp16 the same time). One term of 11 bits puts 1e-4 to 3e-4 of the output
+// between this kernel and fp32 arithmetic, two less than 3e-5, most of it the
+// rounding of the output.
+//
+// In bf16 caches p' has the factor 2^-5: bf16 has the range, and a tile's 32 rows near
+// its end must not overflow. The running O^T carries a factor 2^-k, 2^k >= max_len:
+// sums over all rows stay below the largest value that a row has, so an output that
+// is finite comes out finite. What that costs are the last k bits of outputs near
+// fp32's smallest. A value that is infinite stays so: the second term of a product of
+// its own is never 0, and the merge adds none to an infinite first one.
 //
 // Splits leave (max, sum, accumulator) in the workspace and a second launch joins
 // them by log-sum-exp; a single split without weights writes its output itself.
@@ -62,8 +73,8 @@ constexpr int kMaxSplit = 512;
 
 template <int KIND, int D, int HT>
 struct DecCfg {
-  static constexpr int kCtas = HT == 8 ? 3 : 2;   // per SM
-  static constexpr int kDepth = HT == 8 ? 2 : 3;  // stages per warp
+  static constexpr int kCtas = HT <= 8 ? 3 : 2;   // per SM
+  static constexpr int kDepth = HT <= 8 ? 2 : 3;  // stages per warp
   static constexpr int kEsz = cache_esz(KIND);
   static constexpr int kRowBytes = D * kEsz;                           // 64, 128 or 256
   static constexpr int kBoxBytes = kRowBytes < 128 ? kRowBytes : 128;  // swizzled unit of a row
@@ -72,7 +83,7 @@ struct DecCfg {
   static constexpr int kScaleOff = 2 * kTileBytes;
   static constexpr int kStageBytes = kScaleOff + (cache_8bit(KIND) ? 512 : 0);
   static constexpr int kRingBytes = kWarps * kDepth * kStageBytes;
-  // Merge area (aliases the ring): per warp m[16], l[16], acc[G][D].
+  // Merge area (aliases the ring): per warp m[16], l[16], acc[G][D] (or 8 rows of D + 4).
   static constexpr int kMergeFloats = kWarps * 32 + kWarps * 16 * D;
   static_assert(kMergeFloats * 4 <= kRingBytes, "merge area fits the ring");
   static constexpr int kSmemBytes = kRingBytes + 128;
@@ -178,6 +189,15 @@ __device__ __forceinline__ uint32_t cvt2(uint32_t w) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// Two floats as 16-bit values, cut off instead of rounded, the first in the low half.
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack_cut(float lo, float hi) {
+  if (BF16) return byte_perm(__float_as_uint(lo), __float_as_uint(hi), 0x7632);
+  uint32_t d;
+  asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(d) : "f"(hi), "f"(lo));
+  return d;
+}
+
 template <bool QBF16>
 __device__ __forceinline__ void store_out(const DecodeArgs& a, int64_t i, float o) {
   if (QBF16)
@@ -198,7 +218,9 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
   constexpr bool kF8 = cache_8bit(KIND);
   constexpr bool kMmaBf16 = KIND == kCacheBF16;
   constexpr bool kTwo = HT == 16;
+  constexpr bool kSide = HT == 4;  // second terms in columns 4 to 7
   constexpr float kPScale = kMmaBf16 ? 0.03125f : 32768.f;
+  constexpr uint32_t kCut = kMmaBf16 ? 0xffff0000u : 0xffffe000u;  // what 16 bits hold of an fp32
   constexpr int TK = C::kTK;
   constexpr int KS = D / 16;   // k-steps of Q K^T
   constexpr int MT = D / 16;   // m-tiles of V^T P^T
@@ -317,7 +339,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
     for (int s = 0; s < KS; ++s)
 #pragma unroll
       for (int w = 0; w < 2; ++w) {
-        qa[s][w] = frag(g, s, w);
+        qa[s][w] = frag(kSide ? g & 3 : g, s, w);
         qh[s][w] = kTwo ? frag(g + 8, s, w) : 0u;
       }
     if (QBF16 && kF8) {
@@ -358,6 +380,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
     for (int i = 0; i < 4; ++i) o[mt][i] = o2[mt][i] = 0.f;
   float m_run = -INFINITY, l_run = 0.f, m_run2 = -INFINITY, l_run2 = 0.f;
 
+  const uint32_t side_mask = g < 4 ? 0u : kCut;  // which term this lane gives
   // This thread's place in its head's scores, for own tile 0.
   float* const scores = a.ws_scores + (q0 + g) * a.score_stride + tile_row(0) + (kF8 ? 4 : 2) * c;
   // Rounds -kDepth..-1 only fill the stages: one copy of the code, which a short
@@ -482,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
           if (key_of(nt, e & 1) >= rem) sacc[nt][e] = -INFINITY;
     }
     uint32_t pb[PS][2], pb2[PS][2];    // B fragments of P^T for the 16-key steps
-    uint32_t pl[PS][2], pl2[PS][2];    // what bf16 leaves of them
+    uint32_t pl[PS][2], pl2[PS][2];    // the second terms
     auto head_softmax = [&](int e0, float& m_h, float& l_h, uint32_t (&ph)[PS][2], uint32_t (&plo)[PS][2], float& alpha,
                             float& beta) {
       float mx = -INFINITY;
@@ -496,14 +519,16 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
       for (int nt = 0; nt < NT; ++nt) {
         const float p0 = ex2(sacc[nt][e0] - base), p1 = ex2(sacc[nt][e0 + 1] - base);
         psum += p0 + p1;
-        const float w0 = p0 * vw[nt][0], w1 = p1 * vw[nt][1];
-        if (kMmaBf16) {
-          const uint32_t u0 = __float_as_uint(w0), u1 = __float_as_uint(w1);
-          ph[nt >> 1][nt & 1] = byte_perm(u0, u1, 0x7632);  // the upper halves
-          plo[nt >> 1][nt & 1] = pack_pair<true>(__uint_as_float(u0 | 1u) - __uint_as_float(u0 & 0xffff0000u),
-                                                 __uint_as_float(u1 | 1u) - __uint_as_float(u1 & 0xffff0000u));
-        } else {
-          ph[nt >> 1][nt & 1] = pack_pair<false>(w0, w1);
+        float w0 = p0 * vw[nt][0], w1 = p1 * vw[nt][1];
+        if (kSide) {  // this lane's term
+          w0 -= __uint_as_float(__float_as_uint(w0) & side_mask);
+          w1 -= __uint_as_float(__float_as_uint(w1) & side_mask);
+        }
+        ph[nt >> 1][nt & 1] = pack_cut<kMmaBf16>(w0, w1);
+        if (!kSide) {
+          const uint32_t u0 = __float_as_uint(w0), u1 = __float_as_uint(w1), more = kF8 ? 0u : 1u;  // never 0
+          plo[nt >> 1][nt & 1] = pack_pair<kMmaBf16>(__uint_as_float(u0 | more) - __uint_as_float(u0 & kCut),
+                                                     __uint_as_float(u1 | more) - __uint_as_float(u1 & kCut));
         }
       }
       const float m_new = fmaxf(m_h, mx);
@@ -538,7 +563,11 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
             const uint32_t x = prep8<KIND>(r[2 * u]), y = prep8<KIND>(r[2 * u + 1]);
             const uint32_t a0 = cvt2<KIND, 0>(x), a2 = cvt2<KIND, 1>(x), a1 = cvt2<KIND, 0>(y), a3 = cvt2<KIND, 1>(y);
             mma16816<kMmaBf16>(t[mt + u], a0, a1, a2, a3, pb[sp][0], pb[sp][1]);
-            if (kTwo) mma16816<kMmaBf16>(t2[mt + u], a0, a1, a2, a3, pb2[sp][0], pb2[sp][1]);
+            if (!kSide) mma16816<kMmaBf16>(t[mt + u], a0, a1, a2, a3, pl[sp][0], pl[sp][1]);
+            if (kTwo) {
+              mma16816<kMmaBf16>(t2[mt + u], a0, a1, a2, a3, pb2[sp][0], pb2[sp][1]);
+              if (!kSide) mma16816<kMmaBf16>(t2[mt + u], a0, a1, a2, a3, pl2[sp][0], pl2[sp][1]);
+            }
           }
         }
       } else {
@@ -549,10 +578,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
           uint32_t a0, a1, a2, a3;
           ldsm_x4_t(vt + C::off(row, (2 * mt + (mm & 1)) * 16), a0, a1, a2, a3);
           mma16816<kMmaBf16>(t[mt], a0, a1, a2, a3, pb[sp][0], pb[sp][1]);
-          if (kMmaBf16) mma16816<true>(t[mt], a0, a1, a2, a3, pl[sp][0], pl[sp][1]);
+          if (!kSide) mma16816<kMmaBf16>(t[mt], a0, a1, a2, a3, pl[sp][0], pl[sp][1]);
           if (kTwo) {
             mma16816<kMmaBf16>(t2[mt], a0, a1, a2, a3, pb2[sp][0], pb2[sp][1]);
-            if (kMmaBf16) mma16816<true>(t2[mt], a0, a1, a2, a3, pl2[sp][0], pl2[sp][1]);
+            if (!kSide) mma16816<kMmaBf16>(t2[mt], a0, a1, a2, a3, pl2[sp][0], pl2[sp][1]);
           }
         }
       }
@@ -588,11 +617,8 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
   __syncthreads();  // every stage has been used: the ring is free
   float* mw = reinterpret_cast<float*>(smem);  // [kWarps][16] max
   float* lw = mw + kWarps * 16;                // [kWarps][16] sum
-  float* cm = lw + kWarps * 16;                // [16] the CTA's max
-  float* cl = cm + 16;                         // [16] the CTA's sum
-  float* zs = cl + 16;                         // [16] log2 of the softmax denominator
-  float* ca = zs + 16;                         // [G][D] the CTA's accumulator
-  float* aw = ca + 16 * D;                     // [kWarps][G][D]
+  float* aw = lw + kWarps * 16;                // [kWarps][G][D], or [kWarps][8][kSideD]
+  constexpr int kSideD = D + 4;                // four heads' stores meet no bank twice
   if (c == 0) {
     mw[warp * 16 + g] = m_run;
     lw[warp * 16 + g] = l_run;
@@ -607,7 +633,10 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
     for (int i = 0; i < 4; ++i) {
       const int head = 2 * c + (i & 1), half = i >> 1;
       const int d = 16 * mt + 8 * half + g;
-      if (head < G) aw[(warp * G + head) * D + d] = o[mt][i];
+      if (kSide)
+        aw[(warp * 8 + head) * kSideD + d] = o[mt][i];
+      else if (head < G)
+        aw[(warp * G + head) * D + d] = o[mt][i];
       if (kTwo && head + 8 < G) aw[(warp * G + head + 8) * D + d] = o2[mt][i];
     }
   __syncthreads();
@@ -621,7 +650,15 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float f = ex2(mw[w * 16 + head] - base);
-      acc = fmaf(f, aw[(w * G + head) * D + d], acc);
+      float x;
+      if (kSide) {  // an infinity has no second term
+        x = aw[(w * 8 + head) * kSideD + d];
+        const float rest = aw[(w * 8 + 4 + head) * kSideD + d];
+        x += fabsf(x) < INFINITY ? rest : 0.f;
+      } else {
+        x = aw[(w * G + head) * D + d];
+      }
+      acc = fmaf(f, x, acc);
       L = fmaf(f, lw[w * 16 + head], L);
     }
     if (a.direct) {
@@ -870,8 +907,10 @@ pa_status launch_decode_ht(const DecodePlan& p, const DecodeArgs& a, cudaStream_
 
 template <int KIND, int D, bool QBF16>
 pa_status launch_decode(const DecodePlan& p, const DecodeArgs& a, cudaStream_t st) {
-  // Head tile of 8 rows (groups 1-8) or 16 rows (groups 9-16).
-  return p.G <= 8 ? launch_decode_ht<KIND, D, QBF16, 8>(p, a, st) : launch_decode_ht<KIND, D, QBF16, 16>(p, a, st);
+  // Head tile of 4 rows and their second terms (groups 1-4), 8 rows (5-8) or 16 (9-16).
+  return p.G <= 4   ? launch_decode_ht<KIND, D, QBF16, 4>(p, a, st)
+         : p.G <= 8 ? launch_decode_ht<KIND, D, QBF16, 8>(p, a, st)
+                    : launch_decode_ht<KIND, D, QBF16, 16>(p, a, st);
 }
 
 template <int D>

@@ -164,3 +164,26 @@ def test_infinities_and_nan_reach_what_they_belong_to(fmt, q_dtype, S, weights):
     ok = np.isfinite(ref["out"])
     tol = U[q_dtype] * np.abs(ref["out"]) + (2.0 ** -11 + 2.0 ** -16) * ref["pv"] + 2.0 ** -25
     assert (np.abs(out[ok] - ref["out"][ok]) <= tol[ok]).all()
+
+
+@pytest.mark.parametrize("fmt,q_dtype", [("e4m3", "f16"), ("int8", "bf16"), (None, "f16"), (None, "bf16")])
+@pytest.mark.parametrize("G,H,D", [(1, 2, 64), (4, 2, 128), (3, 1, 64), (5, 1, 128), (8, 2, 64), (9, 1, 128), (16, 1, 64)])
+def test_probabilities_keep_more_bits_than_the_output(fmt, q_dtype, G, H, D):
+    """Probabilities go into the products as two 16-bit terms: what is lost is 2^-10 of 2^-10 (fp16), 2^-7
+    of 2^-7 (bf16 caches), far below half a step of the output even where values cancel; fp32 sums 2^-16."""
+    import torch
+
+    rng = np.random.default_rng(G * D)
+    lens = [3, 40, 1000, 9, 21]
+    c = Cache(rng, 5, H, D, 16, 8, fmt, lens, 1000)
+    if fmt is None and q_dtype == "bf16":
+        for x in (c.k, c.v):
+            x[:] = torch.from_numpy(x).to(torch.bfloat16).double().numpy()
+    d = OnDevice(c, "hnd", q_dtype)
+    q = torch.from_numpy(rng.standard_normal((5, G * H, D))).to("cuda", torch.float16 if q_dtype == "f16" else torch.bfloat16)
+    for weights in (None, rng.random((5, H, 1000)).astype(np.float32)):
+        out, _, _ = decode(d, q, 1000, q_dtype, weights=weights)
+        ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, lens, **c.parts())
+        p = 2.0 ** -14 if fmt is None and q_dtype == "bf16" else 2.0 ** -20
+        tol = U[q_dtype] * np.abs(ref["out"]) + (p + 2.0 ** -16) * ref["pv"] + (2.0 ** -25 if q_dtype == "f16" else 0)
+        assert (np.abs(out - ref["out"]) <= tol).all(), float((np.abs(out - ref["out"]) / tol).max())
