@@ -268,8 +268,9 @@ pa_status pa_decode_kv_fwd(const pa_kv_cache_desc* desc, const void* q, const vo
  *
  * Lengths outside [0, max_seq_len] and block-table entries outside
  * [0, num_pages) are detected on the device and reported by
- * pa_device_status() (codes 0x201, 0x202): the rows involved are not written,
- * and pa_cache_decode reads such rows as zeros.
+ * pa_device_status() (codes 0x201, 0x202). Nothing outside the arrays is
+ * touched, other sequences are as if the call were right, and each call below
+ * says what becomes of the sequence.
  *
  * All calls are asynchronous on `stream`, allocate nothing when given a
  * workspace (16-byte aligned), and can be captured into a CUDA graph; the first
@@ -304,7 +305,10 @@ typedef struct pa_block_cache_desc {
  *
  * seq_lens (int32 [batch]) is required. seq_lens + new tokens beyond
  * max_seq_len is an error of that sequence (code 0x201, nothing of it
- * written). Optional: weights (float, set to 0 for the new rows), positions
+ * written). New rows whose page is wrong (0x202) are written nowhere, and the
+ * length of their sequence stays; what other new rows of it were written lies
+ * behind that length, and the scale of the block around it may have grown.
+ * Optional: weights (float, set to 0 for the new rows), positions
  * (int32, set to start_positions[b] + t, or to the row where start_positions
  * is NULL), seq_lens_out (int32 [batch], the new lengths; not the same memory
  * as seq_lens). Pages that receive rows must belong to one sequence only.

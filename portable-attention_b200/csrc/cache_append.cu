@@ -196,7 +196,20 @@ __global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(c
     if (lane == 0) atomicExch(a.status, kStatusBadSeqLen);
     add = 0;
   }
-  if (a.lens_out && h == 0 && kv == 0 && blk == 0 && lane == 0) a.lens_out[b] = len + add;
+  if (a.lens_out && h == 0 && kv == 0 && blk == 0) {
+    // A sequence some of whose new rows have no page keeps its length.
+    bool wrong = false;
+    if (a.table && add > 0) {
+      const int32_t* pages = a.table + static_cast<int64_t>(b) * a.c.max_pages;
+      const int last = fast_div(a.c.by_page, len + add - 1);
+      for (int i = fast_div(a.c.by_page, len) + lane; i <= last; i += 32) {
+        const int32_t page = pages[i];
+        wrong = wrong || page < 0 || page >= a.c.num_pages;
+      }
+    }
+    wrong = __any_sync(0xffffffffu, wrong);
+    if (lane == 0) a.lens_out[b] = wrong ? len : len + add;
+  }
   const int bs = a.rows_per_block;
   const int64_t r_first = (static_cast<int64_t>(len / bs) + blk) * bs;  // first row of this block
   if (add == 0 || r_first >= static_cast<int64_t>(len) + add) return;
@@ -212,11 +225,13 @@ __global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(c
       (kv ? a.x[1] : a.x[0]) + b * a.x_seq + h * a.x_head + (lo - len + row_l) * a.x_tok + ch * 16;
   uint8_t* const cache = kv ? a.cache[1] : a.cache[0];
   const int rows = hi - lo;
+  // Per-row arrays of the rows that have a page (in 8 bits all have the block's).
   auto set_rows = [&]() {
     if (kv != 0 || !(a.weights || a.positions)) return;
     const int64_t row0 = b * a.c.row_seq + h * a.c.row_head;
     const int p0 = a.positions ? (a.start ? a.start[b] : len) : 0;
     for (int r = lo + lane; r < hi; r += 32) {
+      if (!cache_8bit(KIND) && cache_page(a.c, a.table, b, r, a.status) < 0) continue;
       if (a.weights) a.weights[row0 + r] = 0.f;
       if (a.positions) a.positions[row0 + r] = p0 + (r - len);
     }
@@ -238,7 +253,6 @@ __global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(c
     }
   };
   read(0);  // asked for before the page is known
-  set_rows();
   if (!cache_8bit(KIND)) {
 #pragma unroll
     for (int u = 0; u < kHold; ++u) {
@@ -248,11 +262,13 @@ __global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(c
       if (page < 0) continue;
       *reinterpret_cast<uint4*>(cache + cache_row(a.c, page, h, cache_at(a.c, lo + i)) + ch * 16) = x[u];
     }
+    set_rows();
     return;
   }
   // 8 bits: the block lies in one page.
   const int32_t page = cache_page(a.c, a.table, b, lo, a.status);
   if (page < 0) return;
+  set_rows();
   const int at0 = cache_at(a.c, r0);  // the block's first row inside its page
   float* const sp = (kv ? a.scales[1] : a.scales[0]) + cache_scale(a.c, page, h, at0);
   const bool held = r0 < len;  // earlier rows of this sequence live in the block

@@ -187,3 +187,50 @@ def test_probabilities_keep_more_bits_than_the_output(fmt, q_dtype, G, H, D):
         p = 2.0 ** -14 if fmt is None and q_dtype == "bf16" else 2.0 ** -20
         tol = U[q_dtype] * np.abs(ref["out"]) + (p + 2.0 ** -16) * ref["pv"] + (2.0 ** -25 if q_dtype == "f16" else 0)
         assert (np.abs(out - ref["out"]) <= tol).all(), float((np.abs(out - ref["out"]) / tol).max())
+
+
+def reported(call, text):
+    """Runs the call; the device has to report `text`."""
+    import pa_b200
+    import torch
+    from pa_b200._lib import PaError
+
+    call()
+    torch.cuda.synchronize()
+    with pytest.raises(PaError, match=text):
+        pa_b200.sync_device_status()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("bad", [10 ** 6, -1])
+def test_append_with_a_wrong_page_leaves_its_rows_and_the_length(fmt, bad):
+    """The second page of sequence 1's new rows is wrong; sequence 0 is as ever, sequence 2 is too long."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(81)
+    B, H, D, T, rows = 3, 2, 64, 30, 64
+    lens = [11, 12, 50]
+    c = Cache(rng, B, H, D, 16, 8, fmt, lens, rows)
+    d = OnDevice(c, "hnd")
+    good = c.table.copy()
+    d.table[1, 1] = bad                                     # rows 16 to 31 of sequence 1
+    x = torch.from_numpy(rng.standard_normal((2, B, T, H, D))).to("cuda", torch.float16)
+    w, pos = torch.full((B, H, rows), 7.0, device="cuda"), torch.full((B, H, rows), -5, dtype=torch.int32, device="cuda")
+    out = torch.full((B,), -9, dtype=torch.int32, device="cuda")
+    reported(lambda: pa_b200.cache_append_device(
+        d.desc(H, rows), x[0].data_ptr(), x[1].data_ptr(), T, d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(),
+        weights_ptr=w.data_ptr(), positions_ptr=pos.data_ptr(), seq_lens_out_ptr=out.data_ptr(), **d.kw()), "code 0x20")
+    assert out.tolist() == [41, 12, 50]
+    # What the call means: every block that has a page, none of sequence 2.
+    before = {n: getattr(c, n) if getattr(c, n) is None else getattr(c, n).copy() for n in ("k", "v", "ks", "vs")}
+    xs = x.double().cpu().numpy()
+    append_reference(xs[0], xs[1], c.k, c.v, lens, [T, T, 0], fmt=fmt, **c.parts())
+    for n in ("k", "v", "ks", "vs"):
+        if before[n] is not None:
+            getattr(c, n)[good[1, 1]] = before[n][good[1, 1]]
+    d.check_equal()
+    written = np.zeros((B, 1, rows), bool)
+    written[0, :, 11:41] = written[1, :, 12:16] = written[1, :, 32:42] = True
+    np.testing.assert_array_equal(w.cpu().numpy(), np.broadcast_to(np.where(written, 0.0, 7.0), (B, H, rows)))
+    np.testing.assert_array_equal(pos.cpu().numpy(), np.broadcast_to(np.where(written, np.arange(rows), -5), (B, H, rows)))
