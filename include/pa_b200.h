@@ -360,7 +360,10 @@ pa_status pa_cache_decode(const pa_block_cache_desc* desc, const void* q, const 
  * positions_out (optional): the per-row arrays in the new order, rows behind
  * the new length left as they were; they may be weights and positions
  * themselves. weights must be given. Pages of a sequence that is shrunk must
- * belong to it alone.
+ * belong to it alone. A sequence whose length is wrong, or that would be shrunk
+ * and has a wrong page among those of its rows, is left as it was: its
+ * seq_lens_out is its seq_lens and its kept -1 (weights_out and positions_out,
+ * where they are other arrays, may hold its first `budget` rows as they were).
  */
 pa_status pa_cache_evict_workspace_size(const pa_block_cache_desc* desc, int32_t paged,
                                         int64_t budget, size_t* bytes);

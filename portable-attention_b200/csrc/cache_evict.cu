@@ -106,6 +106,8 @@ struct EvictShared {
   int warp_sum[2][32];
   int total[2];        // this CTA's ranks, read by its cluster
   int digit, left, all;
+  int bad;             // clusters: warps that found a page out of range
+  int found[32];       // this CTA's
 };
 
 // Ranks of the rows that a mask marks (bit i: row i of this thread, group i / 4
@@ -435,7 +437,9 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
       }
     }
   };
-  // One CTA's first rows do not depend on the length: asked for together with it.
+  // One CTA's first rows, and a page to look at for each thread, do not depend on the
+  // length: asked for together with it.
+  const int32_t my_page = C == 1 && a.table && tid < a.c.max_pages ? a.table[static_cast<int64_t>(b) * a.c.max_pages + tid] : 0;
   if (C == 1) fetch(0, a.c.max_len);
   const bool bad = len < 0 || len > a.c.max_len;
   if (h == 0 && rank == 0 && tid == 0) {
@@ -517,6 +521,30 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
     }
   };
 
+  // Whether the warp found a page of the sequence out of range (a cluster's CTAs share
+  // them out). The sequence is then left as it was; that is looked at when the lists
+  // are complete, until when only copies of what it holds have been written.
+  auto look_at_pages = [&]() {
+    int wrong = 0;
+    if (a.table) {
+      const int used = fast_div(a.c.by_page, len - 1) + 1;
+      if (C == 1) wrong = tid < used && (my_page < 0 || my_page >= a.c.num_pages);
+#pragma unroll 1
+      for (int i = rank * T + tid + (C == 1 ? T : 0); i < used; i += C * T) {
+        const int32_t page = a.table[static_cast<int64_t>(b) * a.c.max_pages + i];
+        wrong |= page < 0 || page >= a.c.num_pages;
+      }
+      if (wrong) atomicExch(a.status, kStatusBadPage);
+      wrong = __any_sync(0xffffffffu, wrong);
+    }
+    if (lane == 0) sh.found[tid >> 5] = wrong;
+  };
+  auto leave = [&]() {
+    if (h == 0 && rank == 0 && tid == 0) a.lens_out[b] = len;
+    if (rank == 0 && tid == 0) a.counts[pair] = 0;
+    for (int r = rank * T + tid; r < n; r += C * T) kept[r] = -1;
+  };
+
   // ------------------------------------------------ threshold: radix selection
   // What `move` needs apart from the lists, by one thread or two.
   auto put_aside = [&](int moves) {
@@ -535,6 +563,7 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   if (C == 1 && rounds == 1 && len - n <= kFewRows) {
     rank_keys();
     copy_rows();
+    look_at_pages();
     const int warp = tid >> 5, warps = T >> 5, out = len - n;
     for (int i = 0; i < out; ++i) {
       uint32_t key = 0xffffffffu;
@@ -561,6 +590,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
         if (row_of(k) == gone) live &= ~(1u << k);
       if (tid == 0) sh.own[i] = gone;
       __syncthreads();
+    }
+    if (__any_sync(0xffffffffu, lane < warps && sh.found[lane])) {
+      leave();
+      return;
     }
     if (tid < 32) {
       const int e = lane < out ? sh.own[lane] : 0x7fffffff;
@@ -601,8 +634,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   // A cluster's CTAs add into each other's arrays, so all are cleared up front.
   for (int i = tid; i < (C > 1 ? 4 : 1) * kBins; i += T) (&sh.hist[0][0])[i] = 0;  // own follows hist
   if (C > 1) fetch(row0, row_end);
+  if (tid == 0) sh.bad = 0;
   rank_keys();
   copy_rows();
+  look_at_pages();
   sync_all();
   uint32_t prefix = 0;
   int left = n;  // rows to take among those that match the prefix
@@ -628,6 +663,8 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
         sh.own[i] = 0;
         for (int q = 0; q < C; ++q) cluster_add(&sh.hist[pass][i], q, x);
       }
+      if (pass == 0 && tid < T >> 5 && sh.found[tid])
+        for (int q = 0; q < C; ++q) cluster_add(&sh.bad, q, 1);
     }
     sync_all();
     // Thread t < 256 takes bins 8 t' .. 8 t' + 7 from the top, t' = 255 - t.
@@ -777,6 +814,10 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
     }
   }
   sync_all();  // the lists are complete
+  if (C > 1 ? sh.bad != 0 : __any_sync(0xffffffffu, lane < T >> 5 && sh.found[lane])) {
+    leave();
+    return;
+  }
   for (int k = rank * T + tid; k < hole_all; k += C * T) {
     const int d = holes[k], q = sources[k];
     kept[d] = q;

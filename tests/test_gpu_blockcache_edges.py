@@ -234,3 +234,54 @@ def test_append_with_a_wrong_page_leaves_its_rows_and_the_length(fmt, bad):
     written[0, :, 11:41] = written[1, :, 12:16] = written[1, :, 32:42] = True
     np.testing.assert_array_equal(w.cpu().numpy(), np.broadcast_to(np.where(written, 0.0, 7.0), (B, H, rows)))
     np.testing.assert_array_equal(pos.cpu().numpy(), np.broadcast_to(np.where(written, np.arange(rows), -5), (B, H, rows)))
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("H,n,budget,page_at", [
+    (2, 300, 290, 11), (2, 300, 290, 18),      # few rows go; a page of holes, the last page
+    (3, 303, 299, 3), (3, 700, 120, 0),        # few rows go and the CTA moves them; many go
+    (1, 9000, 4000, 500),                      # a cluster
+])
+def test_evict_with_a_wrong_page_leaves_the_sequence(fmt, H, n, budget, page_at):
+    """Sequence 1 has a wrong page, sequence 3 a wrong length; 0 shrinks as ever and 2 has nothing to lose."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(n + page_at)
+    lens = [n, n, min(budget, 37), n]
+    c = Cache(rng, 4, H, 64, 16, 8, fmt, lens, n)
+    d = OnDevice(c, "hnd")
+    d.table[1, page_at] = c.k.shape[0]
+    d.table[2, 4] = -3                          # behind its rows: not a page of the sequence
+    lens[3] = n + 1
+    d.lens[3] = n + 1
+    w0, p0 = rng.random((4, H, n)).astype(np.float32), np.tile(np.arange(n, dtype=np.int32) + 5, (4, H, 1))
+    for in_place in (False, True):
+        w, pos = torch.from_numpy(w0).cuda(), torch.from_numpy(p0).cuda()
+        w_out = w if in_place else torch.full_like(w, -2.0)
+        p_out = pos if in_place else torch.full_like(pos, -4)
+        nxt = torch.full((4,), n + 5, dtype=torch.int32, device="cuda")
+        lens2 = torch.full((4,), -1, dtype=torch.int32, device="cuda")
+        kept = torch.full((4, H, budget), -7, dtype=torch.int32, device="cuda")
+        reported(lambda: pa_b200.cache_evict_device(
+            d.desc(H, n), d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(), w.data_ptr(), budget, lens2.data_ptr(),
+            kept.data_ptr(), recent=9, sinks=6, positions_ptr=pos.data_ptr(), next_positions_ptr=nxt.data_ptr(),
+            weights_out_ptr=w_out.data_ptr(), positions_out_ptr=p_out.data_ptr(), **d.kw()), "code 0x20")
+        if not in_place:                        # the second call finds sequence 0's cache shrunk once
+            want_w, want_p = w0.copy(), p0.copy()
+            _, want = evict_reference(c.k, c.v, [n, 0, 0, 0], want_w, budget, recent=9, sinks=6, positions=want_p,
+                                      next_positions=[n + 5] * 4, fmt=fmt, **c.parts())
+            d.check_equal()
+        assert lens2.tolist() == [budget, n, min(budget, 37), n + 1]
+        got = kept.cpu().numpy()
+        np.testing.assert_array_equal(got[0], want[0])
+        assert (got[1] == -1).all() and (got[3] == -1).all()
+        np.testing.assert_array_equal(got[2], np.tile(np.r_[0:37, [-1] * (budget - 37)], (H, 1)))
+        np.testing.assert_array_equal(w_out[0, :, :budget].cpu().numpy(), want_w[0, :, :budget])
+        np.testing.assert_array_equal(p_out[0, :, :budget].cpu().numpy(), want_p[0, :, :budget])
+        for b in (1, 3):
+            for got, was, fill in ((w_out[b], w0[b], -2.0), (p_out[b], p0[b], -4)):
+                got = got.cpu().numpy()
+                assert ((got == was) | (not in_place and got == fill)).all()
+                if not in_place:
+                    assert (got[:, budget:] == fill).all()
