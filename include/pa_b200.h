@@ -328,6 +328,9 @@ pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new, co
  * keys everywhere. Table entries behind a sequence's rows may hold anything.
  * `weights` (optional): weights[b][h][j] += the softmax weight of key j, summed
  * over the query heads of kv head h, for every row j of the sequence.
+ * A length above max_seq_len counts as max_seq_len and one below 0 as 0, and
+ * the sequence's weights stay; a row whose page is wrong counts as a key and a
+ * value of zeros, with the weight of such a key.
  * Scales of rows in use must be finite. The cache may span 2^32 times the
  * largest power of two that divides its strides in bytes (16 at least).
  */

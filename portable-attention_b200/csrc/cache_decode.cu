@@ -757,7 +757,7 @@ __global__ void __launch_bounds__(kFinThreads) cache_finish_kernel(const DecodeA
     return;
   }
   const int64_t r0 = static_cast<int64_t>(blockIdx.y - out_ctas) * kRowsPerCta;
-  if (r0 >= len) return;
+  if (r0 >= len || (a.lens && a.lens[b] > a.c.max_len)) return;  // a wrong length: its weights stay
   const int64_t r = r0 + 4 * threadIdx.x;
   const float* sc = a.ws_scores + q0 * a.score_stride + r;
   float4 x[4];

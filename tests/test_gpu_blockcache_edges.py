@@ -285,3 +285,31 @@ def test_evict_with_a_wrong_page_leaves_the_sequence(fmt, H, n, budget, page_at)
                 assert ((got == was) | (not in_place and got == fill)).all()
                 if not in_place:
                     assert (got[:, budget:] == fill).all()
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("rows", [100, 5000])
+def test_decode_with_wrong_lengths_and_pages(fmt, rows):
+    """A length too long counts as the longest, one below 0 as 0, both without weights; a wrong page as zeros."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(rows)
+    B, H, D = 4, 2, 64
+    c = Cache(rng, B, H, D, 16, 8, fmt, [rows] * B, rows)
+    d = OnDevice(c, "hnd")
+    d.lens.copy_(torch.tensor([rows + 1, -1, rows, 60], dtype=torch.int32))
+    d.table[2, 1] = -1
+    q = torch.from_numpy(rng.standard_normal((B, 6, D))).to("cuda", torch.float16)
+    out, lse = torch.empty_like(q), torch.empty((B, 6), device="cuda")
+    w0 = rng.random((B, H, rows)).astype(np.float32)
+    w = torch.from_numpy(w0).cuda()
+    reported(lambda: pa_b200.cache_decode_device(
+        d.desc(6, rows), q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), out.data_ptr(), seq_lens_ptr=d.lens.data_ptr(),
+        lse_ptr=lse.data_ptr(), weights_ptr=w.data_ptr(), **d.kw()), "code 0x20")
+    for x in (c.k, c.v) + ((c.ks, c.vs) if fmt else ()):
+        x[c.table[2, 1]] = 0.0
+    ref = decode_reference(q.double().cpu().numpy(), c.k, c.v, [rows, 0, rows, 60], weights=w0, **c.parts())
+    ref["weights"][:2] = w0[:2]
+    check_decode(ref, out.cpu().numpy(), lse.cpu().numpy(), w.cpu().numpy(), w0)
+    np.testing.assert_array_equal(w[:2].cpu().numpy(), w0[:2])
