@@ -288,7 +288,8 @@ typedef struct pa_block_cache_desc {
 
 /*
  * Append new_len tokens (new_lens[b] where that is given, each in
- * [0, new_len]) behind seq_lens[b] rows of every sequence b. k_new and v_new
+ * [0, new_len]; new_len, the padded width, may then be above max_seq_len)
+ * behind seq_lens[b] rows of every sequence b. k_new and v_new
  * are q_dtype; element (b, token t, head h, d) of both is at
  * b * new_seq_stride + t * new_token_stride + h * new_head_stride + d, with
  * 16-byte aligned bases and strides that are multiples of 8 elements.

@@ -397,7 +397,9 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   clear_error();
   AppendArgs a{};
   PA_TRY(check_cache(desc, {block_table != nullptr, weights || positions, false}, &a.c, "cache append"));
-  if (new_len < 0 || new_len > a.c.max_len) return fail(PA_ERR_INVALID, "cache append: new_len must be in [0, max_seq_len]");
+  // A padded batch may be wider than the cache: each sequence's count is checked on the device.
+  if (new_len < 0 || new_len > (new_lens ? 0x7fffffffLL : a.c.max_len))
+    return fail(PA_ERR_INVALID, "cache append: new_len must be in [0, max_seq_len], or below 2^31 with new_lens");
   if (start_positions && !positions) return fail(PA_ERR_INVALID, "cache append: start_positions without positions");
   if (a.c.B == 0) return PA_OK;
   if (!seq_lens) return fail(PA_ERR_INVALID, "cache append: null seq_lens");
@@ -432,9 +434,9 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   a.T = static_cast<int32_t>(new_len);
   // 16-bit caches have no blocks: 16 rows make an item (eight pieces a lane, or four).
   a.rows_per_block = cache_8bit(a.c.kind) ? a.c.scale_block : 16;
-  // Blocks that T rows starting anywhere can touch; one at least, for seq_lens_out.
-  const int64_t bs = a.rows_per_block;
-  a.blocks = a.T > 0 ? static_cast<int32_t>((a.T + 2 * bs - 2) / bs) : 1;
+  // Blocks that the rows of a sequence, starting anywhere, can touch; one at least, for seq_lens_out.
+  const int64_t bs = a.rows_per_block, most = a.T < a.c.max_len ? a.T : a.c.max_len;
+  a.blocks = most > 0 ? static_cast<int32_t>((most + 2 * bs - 2) / bs) : 1;
   a.items = static_cast<int64_t>(a.c.B) * a.blocks * 2 * a.c.Hkv;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return a.c.D == 128 ? launch_append_kind<128>(a, st) : launch_append_kind<64>(a, st);

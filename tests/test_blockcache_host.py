@@ -287,3 +287,16 @@ def test_numpy_entry_points_refuse_bad_arguments():
                     (dict(seq_lens=[33, 0]), "seq_lens must be in"), (dict(seq_lens=3), "one-dimensional")):
         with pytest.raises(ValueError, match=msg):
             pa_b200.cache_evict(**{**a, "weights": w, "budget": 2, **kw})
+
+
+def test_a_padded_batch_may_be_wider_than_the_cache():
+    """new_len above max_seq_len is refused only where every sequence would take all of it (before any
+    launch: without new_lens the check comes first, with it the next argument's)."""
+    from pa_b200._lib import PaError, check, lib
+
+    d = good_desc()
+    for new_lens, new_len, msg in ((None, 129, "new_len"), (16, 129, "null k_new"), (16, (1 << 31) - 1, "null k_new"),
+                                   (16, 1 << 31, "new_len"), (16, -1, "new_len")):
+        with pytest.raises(PaError, match=msg):
+            check(lib().pa_cache_append(ctypes.byref(d), None, 16, new_len, 2048, 512, 128, new_lens, 16, 16, 16, 16, 16, 16,
+                                        None, None, None, None, None))

@@ -313,3 +313,19 @@ def test_decode_with_wrong_lengths_and_pages(fmt, rows):
     ref["weights"][:2] = w0[:2]
     check_decode(ref, out.cpu().numpy(), lse.cpu().numpy(), w.cpu().numpy(), w0)
     np.testing.assert_array_equal(w[:2].cpu().numpy(), w0[:2])
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+def test_append_of_a_padded_batch_wider_than_the_cache(fmt):
+    import pa_b200
+
+    rng = np.random.default_rng(91)
+    c = Cache(rng, 2, 2, 64, 16, 8, fmt, [10, 0], 32)
+    x = rng.standard_normal((2, 2, 100, 2, 64)).astype(np.float16)
+    w = rng.random((2, 2, 24)).astype(np.float32)                  # arrays of 24 rows
+    new = np.array([5, 24], np.int32)
+    got = pa_b200.cache_append(x[0], x[1], seq_lens=[10, 0], new_lens=new, weights=w, **c.arrays("hnd"))
+    append_reference(x[0], x[1], c.k, c.v, [10, 0], new, fmt=fmt, weights=w, **c.parts())
+    c.check_equal(got, "hnd")
+    assert list(got.seq_lens) == [15, 24]
+    np.testing.assert_array_equal(got.weights, w)
