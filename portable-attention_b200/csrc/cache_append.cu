@@ -96,7 +96,8 @@ pa_status check_cache(const pa_block_cache_desc* d, const CacheUse& use, CacheVi
   v->page_size = static_cast<int32_t>(c.page_size);
   v->num_pages = static_cast<int32_t>(c.num_pages);
   v->max_pages = use.paged ? static_cast<int32_t>(c.max_pages_per_seq) : 1;
-  v->scale_block = esz == 1 ? static_cast<int32_t>(d->scale_block) : 0;
+  // Blocks above a page (of a dense cache) are the page: no sum below passes 32 bits.
+  v->scale_block = esz == 1 ? static_cast<int32_t>(d->scale_block < c.page_size ? d->scale_block : c.page_size) : 0;
   v->max_len = static_cast<int32_t>(c.max_seq_len);
   v->q_bf16 = c.q_dtype == PA_BF16;
   v->kind = c.kv_dtype == PA_FP8_E4M3 ? kCacheE4M3 : c.kv_dtype == PA_I8 ? kCacheI8 : v->q_bf16 ? kCacheBF16 : kCacheF16;
@@ -361,9 +362,8 @@ __global__ void __launch_bounds__(256, kHold == 8 ? 3 : 4) cache_append_kernel(c
 
 template <int KIND, int D, bool QBF16>
 pa_status launch_append(const AppendArgs& a, cudaStream_t st) {
-  auto kern = a.rows_per_block * (D / 8) <= 4 * 32 ? cache_append_kernel<KIND, D, QBF16, 4> : cache_append_kernel<KIND, D, QBF16, 8>;
+  auto kern = a.rows_per_block <= 4 * 32 / (D / 8) ? cache_append_kernel<KIND, D, QBF16, 4> : cache_append_kernel<KIND, D, QBF16, 8>;
   const int64_t grid = (a.items + 7) / 8;
-  if (grid > 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache append: grid too large");
   kern<<<static_cast<unsigned>(grid), 256, 0, st>>>(a);
   PA_CUDA(cudaGetLastError());
   return PA_OK;
@@ -426,8 +426,6 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   a.weights = weights;
   a.positions = positions;
   a.lens_out = seq_lens_out;
-  a.status = device_status_word();
-  if (!a.status) return fail(PA_ERR_CUDA, "device status word unavailable");
   a.x_seq = new_seq_stride * 2;
   a.x_tok = new_token_stride * 2;
   a.x_head = new_head_stride * 2;
@@ -437,7 +435,11 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   // Blocks that the rows of a sequence, starting anywhere, can touch; one at least, for seq_lens_out.
   const int64_t bs = a.rows_per_block, most = a.T < a.c.max_len ? a.T : a.c.max_len;
   a.blocks = most > 0 ? static_cast<int32_t>((most + 2 * bs - 2) / bs) : 1;
-  a.items = static_cast<int64_t>(a.c.B) * a.blocks * 2 * a.c.Hkv;
+  const int64_t per_block = static_cast<int64_t>(a.c.B) * 2 * a.c.Hkv;  // below 2^43
+  if (a.blocks > 8 * 0x7fffffffLL / per_block) return fail(PA_ERR_UNSUPPORTED, "cache append: grid too large");
+  a.items = per_block * a.blocks;
+  a.status = device_status_word();
+  if (!a.status) return fail(PA_ERR_CUDA, "device status word unavailable");
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   return a.c.D == 128 ? launch_append_kind<128>(a, st) : launch_append_kind<64>(a, st);
 }

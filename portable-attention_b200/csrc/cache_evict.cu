@@ -220,7 +220,7 @@ __device__ __forceinline__ void move_block(const EvictArgs& a, int kv, int b, in
   constexpr int kStep = 4 * kRows;     // rows per step: 16 or 32
   const int lane = threadIdx.x & 31;
   const int bs = a.c.scale_block, n = a.budget;
-  const int hi = lo + bs < n ? lo + bs : n;
+  const int hi = n - lo > bs ? lo + bs : n;
   const int cut = n % bs ? n / bs : -1;  // the block whose old scales were put aside
   const int ch = (lane % kPieces) * 16;
   const int32_t* kept = a.kept + pair * n;
@@ -866,7 +866,7 @@ __global__ void __launch_bounds__(32 * kMoveWarps, 4) cache_move_kernel(const Ev
     return;
   }
   const int lo = chunk * a.c.scale_block;
-  const int hi = lo + a.c.scale_block < a.budget ? lo + a.c.scale_block : a.budget;
+  const int hi = a.budget - lo > a.c.scale_block ? lo + a.c.scale_block : a.budget;
   const int32_t* kept = a.kept + pair * a.budget;
   const int src0 = lo + lane < hi ? kept[lo + lane] : lo + lane;  // asked for together with m
   bool moved = src0 != lo + lane;
@@ -876,7 +876,9 @@ __global__ void __launch_bounds__(32 * kMoveWarps, 4) cache_move_kernel(const Ev
 
 struct EvictPlan {
   CacheView c;
-  int64_t list;  // most moves of a (sequence, kv head)
+  int64_t list;    // most moves of a (sequence, kv head)
+  int32_t chunks;  // warps of `move` for each of them (and for keys and values, in 8 bits)
+  bool by_block;   // a chunk is a scale block, else list entries
   size_t bytes;
 };
 
@@ -888,7 +890,15 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
   const int64_t over = p->c.max_len > budget ? p->c.max_len - budget : 0;
   p->list = over < budget ? over : budget;
   p->bytes = pairs * (3 + 2 * static_cast<size_t>(p->list)) * sizeof(int32_t);
-  if (pairs * kMaxCluster > 0x7fffffffu) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
+  int64_t chunks = (p->list + move_entries(p->c.kind) - 1) / move_entries(p->c.kind);
+  if (cache_8bit(p->c.kind)) {
+    const int64_t blocks = (budget + p->c.scale_block - 1) / p->c.scale_block;
+    p->by_block = p->list >= blocks;
+    if (p->by_block) chunks = blocks;
+  }
+  p->chunks = static_cast<int32_t>(chunks);
+  if (pairs * kMaxCluster > 0x7fffffffu || static_cast<int64_t>(pairs) * 2 * chunks / kMoveWarps >= 0x7fffffffLL)
+    return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
   return PA_OK;
 }
 
@@ -898,7 +908,7 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
 // more than kFewRows over the budget, the CTA carries the rows over itself (one row
 // of 2049 in 512 heads: 14.4 us, with a second launch 16.9).
 template <int KIND, int D>
-pa_status launch_evict(EvictArgs a, cudaStream_t st) {
+pa_status launch_evict(EvictArgs a, int32_t chunks, cudaStream_t st) {
   const int64_t pairs = static_cast<int64_t>(a.c.B) * a.c.Hkv;
   int cluster = 1;
   while (cluster < kMaxCluster && pairs * cluster * 2 <= sm_count() && a.c.max_len / (2 * cluster) >= 2048) cluster *= 2;
@@ -926,14 +936,7 @@ pa_status launch_evict(EvictArgs a, cudaStream_t st) {
                                    : threads <= 320 ? cache_select_kernel<8, 320, 4, -1, 0>
                                                     : cache_select_kernel<8, kMaxThreads, 1, -1, 0>, a));
   if (a.list == 0) return PA_OK;
-  int32_t chunks = (a.list + move_entries(KIND) - 1) / move_entries(KIND);
-  if (cache_8bit(KIND)) {
-    const int32_t blocks = (a.budget + a.c.scale_block - 1) / a.c.scale_block;
-    a.by_block = a.list >= blocks;
-    if (a.by_block) chunks = blocks;
-  }
   const int64_t items = pairs * chunks * (cache_8bit(KIND) ? 2 : 1);
-  if (items / kMoveWarps >= 0x7fffffffLL) return fail(PA_ERR_UNSUPPORTED, "cache evict: grid too large");
   // Starts while `select` ends; waits for its memory.
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -946,12 +949,12 @@ pa_status launch_evict(EvictArgs a, cudaStream_t st) {
 }
 
 template <int D>
-pa_status launch_evict_kind(const EvictArgs& a, cudaStream_t st) {
+pa_status launch_evict_kind(const EvictArgs& a, int32_t chunks, cudaStream_t st) {
   switch (a.c.kind) {
     case kCacheF16:
-    case kCacheBF16: return launch_evict<kCacheF16, D>(a, st);  // rows are copied as bits
-    case kCacheE4M3: return launch_evict<kCacheE4M3, D>(a, st);
-    default: return launch_evict<kCacheI8, D>(a, st);
+    case kCacheBF16: return launch_evict<kCacheF16, D>(a, chunks, st);  // rows are copied as bits
+    case kCacheE4M3: return launch_evict<kCacheE4M3, D>(a, chunks, st);
+    default: return launch_evict<kCacheI8, D>(a, chunks, st);
   }
 }
 
@@ -1015,6 +1018,7 @@ extern "C" pa_status pa_cache_evict(const pa_block_cache_desc* desc, void* k_cac
   a.recent = static_cast<int32_t>(recent);
   a.sinks = static_cast<int32_t>(sinks);
   a.list = static_cast<int32_t>(p.list);
+  a.by_block = p.by_block;
   a.vec = ((reinterpret_cast<uintptr_t>(weights) | reinterpret_cast<uintptr_t>(positions) |
             reinterpret_cast<uintptr_t>(weights_out) | reinterpret_cast<uintptr_t>(positions_out)) & 15) == 0 &&
           p.c.row_head % 4 == 0 && p.c.row_seq % 4 == 0;
@@ -1026,7 +1030,7 @@ extern "C" pa_status pa_cache_evict(const pa_block_cache_desc* desc, void* k_cac
   a.counts = reinterpret_cast<int32_t*>(a.cut_scale + pairs * 2);
   a.holes = a.counts + pairs;
   a.sources = a.holes + pairs * p.list;
-  pa_status rc = p.c.D == 128 ? launch_evict_kind<128>(a, st) : launch_evict_kind<64>(a, st);
+  pa_status rc = p.c.D == 128 ? launch_evict_kind<128>(a, p.chunks, st) : launch_evict_kind<64>(a, p.chunks, st);
   scratch_free(own, st);
   return rc;
 }

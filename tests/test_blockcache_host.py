@@ -300,3 +300,25 @@ def test_a_padded_batch_may_be_wider_than_the_cache():
         with pytest.raises(PaError, match=msg):
             check(lib().pa_cache_append(ctypes.byref(d), None, 16, new_len, 2048, 512, 128, new_lens, 16, 16, 16, 16, 16, 16,
                                         None, None, None, None, None))
+
+
+def test_grids_too_large_are_refused_before_any_launch():
+    """Products of accepted sizes that pass 64 bits, or a grid's limit in the second launch only."""
+    from pa_b200._lib import PaError, check, lib
+
+    L, n = lib(), ctypes.c_size_t(0)
+    d = good_desc(paged=True, max_pages_per_seq=1 << 20, scale_block=1)
+    for name, value in (("batch", 65535 * 1024), ("kv_heads", 65535), ("page_size", 2047), ("max_seq_len", (1 << 31) - 65537)):
+        change(d, name, value)
+    change(change(d, "scale_head_stride", 1 << 20), "scale_page_stride", 1 << 20)
+    change(change(d, "row_head_stride", 1 << 31), "row_seq_stride", 1 << 31)
+    change(d, "max_pages_per_seq", 1 << 21)
+    for new_lens, new_len in ((None, 1 << 20), (16, (1 << 31) - 1)):
+        with pytest.raises(PaError, match="grid too large") as err:
+            check(L.pa_cache_append(ctypes.byref(d), 16, 16, new_len, 2048, 512, 128, new_lens, 16, 16, 16, 16, 16, 16,
+                                    None, None, None, None, None))
+        assert err.value.status == 2
+    change(change(d, "batch", 64), "kv_heads", 128)
+    with pytest.raises(PaError, match="grid too large"):
+        check(L.pa_cache_evict_workspace_size(ctypes.byref(d), 1, 1 << 30, ctypes.byref(n)))
+    assert n.value == 0

@@ -329,3 +329,31 @@ def test_append_of_a_padded_batch_wider_than_the_cache(fmt):
     c.check_equal(got, "hnd")
     assert list(got.seq_lens) == [15, 24]
     np.testing.assert_array_equal(got.weights, w)
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_scale_blocks_far_above_the_page_of_a_dense_cache(fmt):
+    """One scale a sequence and head, whatever scale_block says above the page's rows."""
+    import pa_b200
+
+    rng = np.random.default_rng(95)
+    for block in (150, 2 ** 31 - 1):
+        c = Cache(rng, 2, 2, 64, 150, 150, fmt, [100, 3], 150, paged=False)
+        a = {**c.arrays("hnd"), "scale_block": block}
+        x = rng.standard_normal((2, 2, 40, 2, 64)).astype(np.float16)
+        got = pa_b200.cache_append(x[0], x[1], seq_lens=[100, 3], **a)
+        append_reference(x[0], x[1], c.k, c.v, [100, 3], [40, 40], fmt=fmt, **c.parts())
+        c.check_equal(got, "hnd")
+        a = {**c.arrays("hnd"), "scale_block": block}
+        q = rng.standard_normal((2, 4, 64)).astype(np.float16)
+        w0 = np.zeros((2, 2, 150), np.float32)
+        out, lse, w = pa_b200.cache_decode(q, seq_lens=[140, 43], weights=w0, return_lse=True, **a)
+        check_decode(decode_reference(q, c.k, c.v, [140, 43], weights=w0, **c.parts()), out, lse, w, w0)
+        for budget in (137, 64):
+            want_w = w.copy()
+            got = pa_b200.cache_evict(seq_lens=[140, 43], weights=w, budget=budget, recent=5, **a)
+            d = Cache.__new__(Cache)
+            d.__dict__.update({k: v.copy() if isinstance(v, np.ndarray) else v for k, v in c.__dict__.items()})
+            _, kept = evict_reference(d.k, d.v, [140, 43], want_w, budget, recent=5, fmt=fmt, **d.parts())
+            np.testing.assert_array_equal(got.kept, kept)
+            d.check_equal(got, "hnd")
