@@ -146,6 +146,27 @@ def cache_evict_device(desc: BlockCacheDesc, k_cache_ptr, v_cache_ptr, seq_lens_
 _CACHE_DTYPE = {None: np.float16, "e4m3": np.uint8, "int8": np.int8}
 
 
+def _int32(x, name):
+    """``x`` as contiguous int32; values that int32 does not hold are refused, not wrapped or cut off."""
+    x = np.asarray(x)
+    y = np.ascontiguousarray(x.astype(np.int32, casting="unsafe"))
+    if x.dtype != np.int32 and not np.array_equal(x, y):
+        raise ValueError(f"{name} must hold whole numbers of 32 bits")
+    return y
+
+
+def _table(block_table):
+    """A block table as int32. Entries behind the rows in use may hold anything: one that int32 does not
+    hold becomes -1, which is no page."""
+    t = np.asarray(block_table)
+    if t.dtype == np.int32:
+        return np.ascontiguousarray(t)
+    ok = (t >= -(2 ** 31)) & (t < 2 ** 31)
+    out = np.full(t.shape, -1, np.int32)
+    out[ok] = _int32(t[ok], "block_table")
+    return out
+
+
 def _check_arrays(key_cache, value_cache, k_scales, v_scales, block_table, batch, *, layout,
                   kv_format, scale_block):
     """Contiguous cache, scale and table arrays, and the scale block they imply."""
@@ -179,7 +200,7 @@ def _check_arrays(key_cache, value_cache, k_scales, v_scales, block_table, batch
             raise ValueError(f"scales must have shape {shape}, got {ks.shape} and {vs.shape}")
     bt = None
     if block_table is not None:
-        bt = np.ascontiguousarray(block_table, dtype=np.int32)
+        bt = _table(block_table)
         if bt.ndim != 2 or bt.shape[0] != batch:
             raise ValueError(f"block_table must be (batch, max_pages_per_seq), got {bt.shape}")
     elif k.shape[0] < batch:
@@ -189,7 +210,7 @@ def _check_arrays(key_cache, value_cache, k_scales, v_scales, block_table, batch
 
 
 def _per_sequence(x, name, batch):
-    x = np.ascontiguousarray(x, dtype=np.int32)
+    x = _int32(x, name)
     if x.shape != (batch,):
         raise ValueError(f"{name} must have shape ({batch},), got {x.shape}")
     return x
@@ -198,7 +219,7 @@ def _per_sequence(x, name, batch):
 def _per_row(x, name, dtype, batch, heads, rows):
     if x is None:
         return None
-    x = np.ascontiguousarray(x, dtype=dtype)
+    x = _int32(x, name) if dtype == np.int32 else np.ascontiguousarray(x, dtype=dtype)
     if x.ndim != 3 or x.shape[:2] != (batch, heads) or x.shape[2] < rows:
         raise ValueError(f"{name} must be (batch, kv_heads, at least {rows} rows), got {x.shape}")
     return x

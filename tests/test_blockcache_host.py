@@ -322,3 +322,30 @@ def test_grids_too_large_are_refused_before_any_launch():
     with pytest.raises(PaError, match="grid too large"):
         check(L.pa_cache_evict_workspace_size(ctypes.byref(d), 1, 1 << 30, ctypes.byref(n)))
     assert n.value == 0
+
+
+def test_numpy_entry_points_refuse_numbers_that_int32_does_not_hold():
+    """2^32 + 3 is no length of 3, and 3.5 none either."""
+    import pa_b200
+
+    a = {**arrays(), "block_table": TABLE}
+    x, w = np.zeros((2, 1, 2, 64), np.float16), np.zeros((2, 2, 32), np.float32)
+    lens = np.array([3, 4])
+    for bad in ([2 ** 32 + 3, 4], [3.5, 4.0], np.array([2 ** 63 + 3, 4], np.uint64), [float("nan"), 1.0]):
+        for call in (lambda: pa_b200.cache_append(x, x, seq_lens=bad, **a), lambda: pa_b200.cache_append(x, x, seq_lens=lens, new_lens=bad, **a),
+                     lambda: pa_b200.cache_decode(x[:, 0], seq_lens=bad, **a),
+                     lambda: pa_b200.cache_evict(seq_lens=bad, weights=w, budget=2, **a),
+                     lambda: pa_b200.cache_evict(seq_lens=lens, weights=w, budget=2, next_positions=bad, **a),
+                     lambda: pa_b200.cache_append(x, x, seq_lens=lens, positions=np.full((2, 2, 32), bad[0]), **a)):
+            with np.errstate(invalid="ignore"), pytest.raises(ValueError, match="32 bits"):
+                call()
+
+
+def test_table_entries_that_int32_does_not_hold_are_no_pages():
+    from pa_b200.blockcache import _table
+
+    t = _table(np.array([[0, 2 ** 32 + 1], [2 ** 63 - 1, -(2 ** 40)]]))
+    assert t.dtype == np.int32 and t.tolist() == [[0, -1], [-1, -1]]
+    assert _table(np.array([[7, 2 ** 64 - 1]], np.uint64)).tolist() == [[7, -1]]
+    with pytest.raises(ValueError, match="32 bits"):
+        _table([[0.5, 1.0]])
