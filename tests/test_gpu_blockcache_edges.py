@@ -357,3 +357,115 @@ def test_scale_blocks_far_above_the_page_of_a_dense_cache(fmt):
             _, kept = evict_reference(d.k, d.v, [140, 43], want_w, budget, recent=5, fmt=fmt, **d.parts())
             np.testing.assert_array_equal(got.kept, kept)
             d.check_equal(got, "hnd")
+
+
+@pytest.mark.parametrize("fmt", FORMATS)
+@pytest.mark.parametrize("D,page,block,layout", [(128, 16, 16, "hnd"), (128, 128, 64, "nhd"), (64, 128, 128, "hnd"), (128, 8, 2, "nhd")])
+@pytest.mark.parametrize("spare", [0, 3, 9, 700, 20000])
+def test_evict_of_a_few_rows_from_descriptors_of_any_width(fmt, D, page, block, layout, spare):
+    """1 to 8 rows over the budget, in arrays of `spare` rows more than the longest sequence: the CTA that
+    selects moves the rows where no sequence can have more than eight to lose, else a second launch does."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(D + page + spare)
+    B, H, budget = 3, 2, 333
+    lens = [budget + 5, budget + 1, budget + 8 - min(spare, 8)]
+    rows = max(lens) + spare
+    c = Cache(rng, B, H, D, page, block, fmt, lens, rows)
+    d = OnDevice(c, layout)
+    w0 = np.round(rng.exponential(size=(B, H, rows)) * 30).astype(np.float32) / 30
+    w = torch.from_numpy(w0).cuda()
+    pos = torch.arange(rows, dtype=torch.int32, device="cuda").expand(B, H, rows).contiguous()
+    lens2, kept = torch.empty_like(d.lens), torch.empty((B, H, budget), dtype=torch.int32, device="cuda")
+    pa_b200.cache_evict_device(d.desc(H, rows), d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(), w.data_ptr(), budget,
+                               lens2.data_ptr(), kept.data_ptr(), recent=20, sinks=3, positions_ptr=pos.data_ptr(),
+                               next_positions_ptr=d.lens.data_ptr(), weights_out_ptr=w.data_ptr(), positions_out_ptr=pos.data_ptr(),
+                               **d.kw())
+    torch.cuda.synchronize()
+    pa_b200.sync_device_status()
+    want_w, want_p = w0.copy(), np.broadcast_to(np.arange(rows, dtype=np.int32), (B, H, rows)).copy()
+    want_len, want = evict_reference(c.k, c.v, lens, want_w, budget, recent=20, sinks=3, positions=want_p,
+                                     next_positions=lens, fmt=fmt, **c.parts())
+    np.testing.assert_array_equal(kept.cpu().numpy(), want)
+    np.testing.assert_array_equal(w.cpu().numpy(), want_w)
+    np.testing.assert_array_equal(pos.cpu().numpy(), want_p)
+    assert lens2.tolist() == list(want_len)
+    d.check_equal()
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "int8"])
+def test_append_of_bf16_near_the_ends_of_its_range(fmt):
+    """Scales up to 2^121 and down to 2^-100; earlier rows 2^200 below are coded to 0."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(97)
+    c = Cache(rng, 1, 2, 64, 16, 8, fmt, [4], 64)
+    d = OnDevice(c, "nhd", "bf16")
+    x = rng.standard_normal((2, 1, 40, 2, 64))
+    x[0, 0, :12] *= 2.0 ** 125
+    x[0, 0, 12:20] *= 2.0 ** -98
+    x[1, 0, 20:] *= 2.0 ** -126
+    t = torch.from_numpy(x).to("cuda", torch.bfloat16)
+    assert bool(torch.isfinite(t).all())
+    pa_b200.cache_append_device(d.desc(2, 64, "bf16"), t[0].data_ptr(), t[1].data_ptr(), 40, d.k.data_ptr(), d.v.data_ptr(),
+                                d.lens.data_ptr(), **d.kw())
+    torch.cuda.synchronize()
+    pa_b200.sync_device_status()
+    xs = t.double().cpu().numpy()
+    append_reference(xs[0], xs[1], c.k, c.v, [4], [40], fmt=fmt, **c.parts())
+    d.check_equal()
+
+
+def pool_high(reset=False):
+    """Most bytes in use of the device's default pool since the last reset."""
+    import ctypes
+
+    cuda = ctypes.CDLL("libcuda.so.1")
+    dev, pool, value = ctypes.c_int(0), ctypes.c_void_p(), ctypes.c_uint64(0)
+    import torch
+
+    assert cuda.cuDeviceGet(ctypes.byref(dev), torch.cuda.current_device()) == 0
+    assert cuda.cuDeviceGetDefaultMemPool(ctypes.byref(pool), dev) == 0
+    used_high = 8                                     # CU_MEMPOOL_ATTR_USED_MEM_HIGH
+    if reset:
+        assert cuda.cuMemPoolSetAttribute(pool, used_high, ctypes.byref(value)) == 0
+    assert cuda.cuMemPoolGetAttribute(pool, used_high, ctypes.byref(value)) == 0
+    return value.value
+
+
+def test_the_pool_is_used_without_workspaces_and_not_with_them():
+    """The default pool keeps what it once had, so free memory says nothing: its most bytes in use do."""
+    import pa_b200
+    import torch
+
+    rng = np.random.default_rng(99)
+    c = Cache(rng, 2, 2, 64, 16, 16, "int8", [4000, 9], 4200)
+    d = OnDevice(c, "hnd")
+    desc = d.desc(4, 4200)
+    q, x = torch.randn((2, 4, 64), device="cuda").half(), torch.randn((2, 2, 8, 2, 64), device="cuda").half()
+    out, w = torch.empty_like(q), torch.zeros((2, 2, 4200), device="cuda")
+    lens2, lens3 = torch.empty_like(d.lens), torch.empty_like(d.lens)
+    kept = torch.empty((2, 2, 3000), dtype=torch.int32, device="cuda")
+    n1, n2 = pa_b200.cache_decode_workspace_size(desc, True, True), pa_b200.cache_evict_workspace_size(desc, True, 3000)
+    ws = torch.empty((max(n1, n2),), dtype=torch.uint8, device="cuda")
+
+    def used(ws1, ws2):
+        torch.cuda.synchronize()
+        base = pool_high(reset=True)
+        for _ in range(3):
+            pa_b200.cache_append_device(desc, x[0].data_ptr(), x[1].data_ptr(), 8, d.k.data_ptr(), d.v.data_ptr(), d.lens.data_ptr(),
+                                        weights_ptr=w.data_ptr(), seq_lens_out_ptr=lens2.data_ptr(), **d.kw())
+            pa_b200.cache_decode_device(desc, q.data_ptr(), d.k.data_ptr(), d.v.data_ptr(), out.data_ptr(),
+                                        seq_lens_ptr=lens2.data_ptr(), weights_ptr=w.data_ptr(), workspace=ws1, **d.kw())
+            pa_b200.cache_evict_device(desc, d.k.data_ptr(), d.v.data_ptr(), lens2.data_ptr(), w.data_ptr(), 3000, lens3.data_ptr(),
+                                       kept.data_ptr(), weights_out_ptr=w.data_ptr(), workspace=ws2, **d.kw())
+        torch.cuda.synchronize()
+        return pool_high() - base
+
+    used((None, 0), (None, 0))
+    assert used((ws.data_ptr(), n1), (ws.data_ptr(), n2)) == 0
+    assert used((None, 0), (ws.data_ptr(), n2)) >= n1          # the count sees what the calls take themselves
+    assert used((ws.data_ptr(), n1), (None, 0)) >= n2
+    pa_b200.sync_device_status()
