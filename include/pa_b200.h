@@ -42,8 +42,9 @@ enum {
 
 /* Element types. PA_FP8_E4M3 is the OCP FP8 E4M3 format ("e4m3fn": 1 sign,
  * 4 exponent bits with bias 7, 3 mantissa bits, no infinities, 0x7f / 0xff
- * NaN, largest finite 448); it is accepted only as a decode cache type. PA_I8
- * is a signed byte (codes -127..127), accepted only by the pa_cache_* calls. */
+ * NaN, largest finite 448); it is accepted only as a key/value cache type
+ * (pa_decode_kv_fwd, pa_cache_*). PA_I8 is a signed byte (codes -127..127),
+ * accepted only by the pa_cache_* calls. */
 enum { PA_F16 = 1, PA_BF16 = 2, PA_F32 = 3, PA_F64 = 4, PA_BOOL = 5, PA_FP8_E4M3 = 6, PA_I8 = 7 };
 
 /* Mask kinds: none, boolean keep-mask (1 byte per element, nonzero = keep),
@@ -279,7 +280,7 @@ pa_status pa_decode_kv_fwd(const pa_kv_cache_desc* desc, const void* q, const vo
  */
 typedef struct pa_block_cache_desc {
   pa_kv_cache_desc cache;
-  int64_t scale_block;       /* keys per scale */
+  int64_t scale_block;       /* keys per scale (above page_size: page_size) */
   int64_t scale_head_stride; /* float elements between kv heads */
   int64_t scale_page_stride; /* float elements between pages */
   int64_t row_head_stride;   /* elements between kv heads of a per-row array */

@@ -12,7 +12,8 @@ namespace pa {
 // Element kinds of a cache (template parameter of every kernel).
 enum : int { kCacheF16 = 0, kCacheBF16 = 1, kCacheE4M3 = 2, kCacheI8 = 3 };
 
-// Division of 0 <= n < 2^31 by a fixed d >= 1 as a high product, an add and a shift.
+// Division of 0 <= n < 2^31 by a fixed d >= 1 as a high product, an add and a shift
+// (Granlund and Montgomery, Division by Invariant Integers using Multiplication, 1994).
 struct FastDiv {
   uint32_t d, mul, shift;
 };

@@ -15,10 +15,12 @@
 // read once; larger blocks are read again. Magnitudes compare as integers two at
 // a time, and where s' is a power of two in fp16's range the coding is packed
 // fp16 arithmetic that rounds once. The new rows are asked for before the page is
-// known. 8 x 4096 tokens of 8 x 128 fp16 to e4m3 in 16-row blocks: 42.5 us, 4.7
-// TB/s of the 204 MB that must move (72 % of the measured copy rate), with 24 warps
+// known. 8 x 4096 tokens of 8 x 128 fp16 to e4m3 in 16-row blocks: 41.3 us, 4.9
+// TB/s of the 204 MB that must move (75 % of the measured copy rate), with 24 warps
 // an SM; bound by the chain length -> rows and page -> codes at that occupancy
-// (issue slots half used). One token in each of 64 sequences: 6.3 us, the host call.
+// (issue slots half used). To fp16: 47.3 us for 268 MB (5.7 TB/s). Larger blocks have
+// fewer warps and read their rows again: 128 rows 65 us, 1024 120, 4096 416. One token
+// in each of 64 sequences: 6.3 us, the host call.
 #include <math.h>
 
 #include <cmath>

@@ -34,7 +34,7 @@
 // term, 638 with two; the same time in fp16). Larger groups take products of their
 // own (16 x 8 x 32768 e4m3: 8 heads 183 and 196 us, 16 heads 235 and 274; 32 x 8 x
 // 4097 fp16 the same time). One term of 11 bits puts 1e-4 to 3e-4 of the output
-// between this kernel and fp32 arithmetic, two less than 3e-5, most of it the
+// between this kernel and fp32 arithmetic, two less than 7e-5, all of it the
 // rounding of the output.
 //
 // In bf16 caches p' has the factor 2^-5: bf16 has the range, and a tile's 32 rows near
@@ -49,11 +49,12 @@
 // With weights every score goes to the workspace (4 bytes a row and query head)
 // and the second launch turns it into exp(s - lse) once the sums are known.
 //
-// 64 x 8 x 32768 x 128 e4m3 in 16-row pages: 637 us, 6.75 TB/s (a read-only stream
-// exceeds the measured copy rate), up to 730 us where the power cap lowers the SM
-// clock (640 instructions a tile and warp, half of the issue slots). 32 x 8 x 4097
-// x 128 fp16: 82 us, with weights 98 (scores 2, second launch 10). 131071 e4m3 keys
-// of one sequence with weights: 61 us for 277 MB, a single wave of CTAs. Three CTAs
+// 64 x 8 x 32768 x 128 e4m3 in 16-row pages: 638 us, 6.75 TB/s (a read-only stream
+// exceeds the measured copy rate), up to 737 us (5.84 TB/s) where the power cap lowers
+// the SM clock: it is bound by memory at full clock only (650 instructions a tile and
+// warp, half of the issue slots). 32 x 8 x 4097 x 128 fp16: 82 us, with weights 97-101
+// (scores 2, second launch 10). 131071 e4m3 keys of one sequence with weights: 58-61
+// us for 277 MB, 50 of them a single wave of CTAs, then the second launch. Three CTAs
 // an SM with two stages a warp against two with three: 661-750 and 722-810 us.
 #include <math.h>
 
@@ -682,6 +683,8 @@ __global__ void __launch_bounds__(kThreads, DecCfg<KIND, D, HT>::kCtas) cache_de
 // of kRowsPerCta rows, four a thread.
 constexpr int kFinThreads = 256;
 constexpr int kRowsPerCta = 4 * kFinThreads;
+// E = 256 against E = 32: 8 splits with weights 10.6 and 12.7 us (5 x 8 x 1023 int8), 8
+// to 16 without 8.4 and 8.4, 32 10.6 and 10.4, 55 14.5 and 12.6 (8 x 8192 e4m3).
 constexpr int kFewSplits = 16;
 
 template <int D, bool QBF16, int E>

@@ -11,18 +11,17 @@
 // first hole).
 //
 // Two launches, the second started while the first ends (one where few rows can
-// go). `select`: a (sequence,
-// kv head) is one CTA, or a cluster of up to eight where there are few of them.
-// Each thread holds eight or sixteen rows' keys in registers, four neighbours at a
-// time so that a warp's reads are whole lines (longer shares are read again in
-// rounds). The threshold key is found by radix
-// selection, digits of 11, 11 and 10 bits counted in shared memory (a cluster's
-// CTAs add their counts into each other's memory); it stops as soon as a digit's
-// rows are all taken. Ranks of ties, holes and sources are prefix sums over the
-// threads. Holes and sources go to two lists in the workspace, and the per-row
-// arrays are written. `move` carries the rows over: in 16 bits a warp takes 32
-// list entries. The call reads 8 bytes a row, writes 12 bytes a kept row and moves
-// what must move.
+// go). `select`: a (sequence, kv head) is one CTA, or a cluster of up to eight where
+// there are few of them. Each thread holds eight or sixteen rows' keys in registers,
+// four neighbours at a time so that a warp's reads are whole lines (longer shares are
+// read again in rounds: over 16384 rows a CTA for every digit and every rank, three
+// to six times in all). The threshold key is found by radix selection, digits of 11,
+// 11 and 10 bits counted in shared memory (a cluster's CTAs add their counts into
+// each other's memory); it stops as soon as a digit's rows are all taken. Ranks of
+// ties, holes and sources are prefix sums over the threads. Holes and sources go to
+// two lists in the workspace, and the per-row arrays are written. `move` carries the
+// rows over: in 16 bits a warp takes 32 list entries. The call reads 8 bytes a row,
+// writes 12 bytes a kept row and moves what must move.
 //
 // In 8-bit caches a warp owns the keys or the values of a whole scale block, the
 // one whose first hole is among the eight list entries it looks at; kept[] tells
@@ -31,11 +30,16 @@
 // possibly sources at or above it: `select` puts its old scales aside, since
 // `move` changes them while other warps read from it.
 //
-// One row over the budget of 2048 in 512 heads (e4m3): 14.4 us, nearly all latency
-// (keys, the minimum, then the move's chain list -> block -> page and scale -> row;
-// 22 us when digits were counted and rows moved by a second launch). 128 heads of up to 8191 fp16 rows to 3001: 44 us for 137
-// MB. 8 heads of 131071 int8 rows to 16384: 61 us for 71 MB, half of it selection
-// on the clusters' 64 SMs, half the moves' look-ups and recoding.
+// One row over the budget of 2048 in 512 heads (e4m3): 14.7 us for 21.8 MB, nearly
+// all latency (keys, the minimum, then the move's chain list -> block -> page and
+// scale -> row), where no sequence can have more than eight rows to lose (max_seq_len
+// <= budget + 8, and 2560 at most). Wider descriptors pay for their width: CTAs of
+// max_seq_len rows, the keys of all of them read before the length is known, and a
+// second launch with warps for as many moves as there could be: max_seq_len 4096
+// 41.7 us, 8192 53.7, 32768 71.4 for the same row; 4097 rows to 4096 29.4. 128 heads
+// of up to 8191 fp16 rows to 3001: 44 us for 137 MB (19 selection, 23 moves). 8 heads
+// of 131071 int8 rows to 16384: 63 us for 71 MB (37 selection on the clusters' 64
+// SMs, 26 moves, bound by look-ups and recoding).
 #include <math.h>
 
 #include "cache.cuh"
@@ -47,7 +51,12 @@ constexpr int kBins = 2048;     // digits of 11 bits (the last: 10)
 constexpr int kScanThreads = 256;
 constexpr int kMaxThreads = 1024;
 constexpr int kMaxCluster = 8;  // portable cluster size
-constexpr int kFewRows = 8;     // rows to evict that are picked one by one
+// Rows to evict that are picked one by one, about 2.7 us each for 512 heads of 2048
+// rows, instead of by counting digits. One row: 14.7 us picked and moved by the same
+// CTA, 22.9 by digits; eight 33.6 and 42.1. Where a second launch moves them (8192
+// rows a head in the arrays): one row 53.7 and 70.2, eight 82.4 and 82.7, sixteen 113
+// and 93.
+constexpr int kFewRows = 8;
 
 struct EvictArgs {
   CacheView c;
@@ -384,7 +393,8 @@ __device__ __forceinline__ void move_entries_of(const EvictArgs& a, int64_t pair
 // kThreads and kCtas bound the registers: 1024 threads, or four CTAs of 256 to 320
 // for many short sequences, so that 512 of them run at once.
 // kMoveKind >= 0: at most kFewRows rows go, and the CTA carries the rows over too
-// (the rest of the kernel is then not reached).
+// (the rest of the kernel is then not reached, which the compiler would report).
+#pragma nv_diagnostic push
 #pragma nv_diag_suppress 128
 template <int kKeys, int kThreads, int kCtas, int kMoveKind, int kMoveD>
 __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const EvictArgs a) {
@@ -845,8 +855,12 @@ __global__ void __launch_bounds__(kThreads, kCtas) cache_select_kernel(const Evi
   put_aside(hole_all);
 }
 
+#pragma nv_diagnostic pop
+
 // The rows of 8-bit caches where moves can be as many as blocks: a warp has one
-// block's keys or values. Else by list entries.
+// block's keys or values. Else by list entries. (128 heads to 3001 rows of e4m3, 188
+// blocks: 40 moves 37.4 us by entries and 36.3 by blocks, 100 moves 46.5 and 47.1,
+// 188 57.2 and 54.8, 500 75.1 and 68.3.)
 template <int KIND, int D>
 __global__ void __launch_bounds__(32 * kMoveWarps, 4) cache_move_kernel(const EvictArgs a, int32_t chunks, int64_t items) {
   __shared__ MoveSlot all_slots[kMoveWarps][32];
@@ -903,10 +917,11 @@ pa_status plan_evict(const pa_block_cache_desc* d, bool paged, int64_t budget, E
 }
 
 // A CTA per (sequence, kv head), or a cluster of 2, 4 or 8 while each CTA then has
-// an SM and 2048 rows (128 heads of 8191 rows: 44.0 us alone, 49.0 in pairs); threads for eight rows each, sixteen
-// where 1024 threads of eight would need a second round. Where no sequence can be
-// more than kFewRows over the budget, the CTA carries the rows over itself (one row
-// of 2049 in 512 heads: 14.4 us, with a second launch 16.9).
+// an SM and 2048 rows (128 heads of 8191 rows: 44.0 us alone, 49.0 in pairs);
+// threads for eight rows each, sixteen where 1024 threads of eight would need a
+// second round. Where max_seq_len lets no sequence be more than kFewRows over the
+// budget, the CTA carries the rows over itself (one row of 2049 in 512 heads: 14.4 us,
+// with a second launch 16.9).
 template <int KIND, int D>
 pa_status launch_evict(EvictArgs a, int32_t chunks, cudaStream_t st) {
   const int64_t pairs = static_cast<int64_t>(a.c.B) * a.c.Hkv;
