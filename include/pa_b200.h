@@ -313,7 +313,7 @@ typedef struct pa_block_cache_desc {
  * Optional: weights (float, set to 0 for the new rows), positions
  * (int32, set to start_positions[b] + t, or to the row where start_positions
  * is NULL), seq_lens_out (int32 [batch], the new lengths; not the same memory
- * as seq_lens). Pages that receive rows must belong to one sequence only.
+ * as seq_lens, new_lens or start_positions). Pages that receive rows must belong to one sequence only.
  */
 pa_status pa_cache_append(const pa_block_cache_desc* desc, const void* k_new, const void* v_new,
                           int64_t new_len, int64_t new_seq_stride, int64_t new_token_stride,
@@ -361,7 +361,8 @@ pa_status pa_cache_decode(const pa_block_cache_desc* desc, const void* q, const 
  * recent + sinks <= budget, budget >= 1.
  * Outputs: kept (int32, dense [batch][kv_heads][budget]): the row that each
  * row held before, -1 behind a shorter sequence; seq_lens_out (int32 [batch]):
- * min(length, budget), not the same memory as seq_lens; weights_out and
+ * min(length, budget), not the same memory as seq_lens or next_positions;
+ * weights_out and
  * positions_out (optional): the per-row arrays in the new order, rows behind
  * the new length left as they were; they may be weights and positions
  * themselves. weights must be given. Pages of a sequence that is shrunk must

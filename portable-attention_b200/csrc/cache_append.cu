@@ -406,6 +406,8 @@ extern "C" pa_status pa_cache_append(const pa_block_cache_desc* desc, const void
   if (a.c.B == 0) return PA_OK;
   if (!seq_lens) return fail(PA_ERR_INVALID, "cache append: null seq_lens");
   if (seq_lens_out == seq_lens) return fail(PA_ERR_INVALID, "cache append: seq_lens_out must not be seq_lens");
+  if (seq_lens_out && (seq_lens_out == new_lens || seq_lens_out == start_positions))
+    return fail(PA_ERR_INVALID, "cache append: seq_lens_out must not be new_lens or start_positions");
   if (new_len > 0) {
     PA_TRY(check_cache_ptrs(a.c, k_cache, v_cache, k_scales, v_scales, "cache append"));
     if (!k_new || !v_new) return fail(PA_ERR_INVALID, "cache append: null k_new or v_new");

@@ -1006,6 +1006,7 @@ extern "C" pa_status pa_cache_evict(const pa_block_cache_desc* desc, void* k_cac
   if (!seq_lens || !weights || !seq_lens_out || !kept)
     return fail(PA_ERR_INVALID, "cache evict: null seq_lens, weights, seq_lens_out or kept pointer");
   if (seq_lens_out == seq_lens) return fail(PA_ERR_INVALID, "cache evict: seq_lens_out must not be seq_lens");
+  if (seq_lens_out == next_positions) return fail(PA_ERR_INVALID, "cache evict: seq_lens_out must not be next_positions");
   PA_TRY(check_cache_ptrs(p.c, k_cache, v_cache, k_scales, v_scales, "cache evict"));
   if (workspace && workspace_bytes < p.bytes)
     return fail(PA_ERR_INVALID, "cache evict: workspace smaller than pa_cache_evict_workspace_size");

@@ -349,3 +349,21 @@ def test_table_entries_that_int32_does_not_hold_are_no_pages():
     assert _table(np.array([[7, 2 ** 64 - 1]], np.uint64)).tolist() == [[7, -1]]
     with pytest.raises(ValueError, match="32 bits"):
         _table([[0.5, 1.0]])
+
+
+def test_lengths_are_not_written_over_what_the_call_reads():
+    """seq_lens_out in the memory of new_lens, start_positions or next_positions: other blocks read those."""
+    from pa_b200._lib import PaError, check, lib
+
+    L, d = lib(), good_desc()
+
+    def append(new_lens, start, lens_out):
+        check(L.pa_cache_append(ctypes.byref(d), 16, 16, 4, 2048, 512, 128, new_lens, 16, 16, 16, 16, 16, 32, None, 16, start,
+                                lens_out, None))
+
+    for args in ((48, None, 48), (48, 64, 64)):
+        with pytest.raises(PaError, match="seq_lens_out must not be") as err:
+            append(*args)
+        assert err.value.status == 1
+    with pytest.raises(PaError, match="seq_lens_out must not be"):
+        check(L.pa_cache_evict(ctypes.byref(d), 16, 16, 16, 16, 16, 16, 16, 16, 48, 10, 2, 1, None, None, 48, 16, 16, 1 << 30, None))
