@@ -149,8 +149,11 @@ _CACHE_DTYPE = {None: np.float16, "e4m3": np.uint8, "int8": np.int8}
 def _int32(x, name):
     """``x`` as contiguous int32; values that int32 does not hold are refused, not wrapped or cut off."""
     x = np.asarray(x)
-    y = np.ascontiguousarray(x.astype(np.int32, casting="unsafe"))
-    if x.dtype != np.int32 and not np.array_equal(x, y):
+    if x.dtype == np.int32:
+        return np.ascontiguousarray(x)
+    with np.errstate(invalid="ignore"):
+        y = np.ascontiguousarray(x.astype(np.int32))
+    if not np.array_equal(x, y):
         raise ValueError(f"{name} must hold whole numbers of 32 bits")
     return y
 

@@ -337,7 +337,7 @@ def test_numpy_entry_points_refuse_numbers_that_int32_does_not_hold():
                      lambda: pa_b200.cache_evict(seq_lens=bad, weights=w, budget=2, **a),
                      lambda: pa_b200.cache_evict(seq_lens=lens, weights=w, budget=2, next_positions=bad, **a),
                      lambda: pa_b200.cache_append(x, x, seq_lens=lens, positions=np.full((2, 2, 32), bad[0]), **a)):
-            with np.errstate(invalid="ignore"), pytest.raises(ValueError, match="32 bits"):
+            with pytest.raises(ValueError, match="32 bits"):
                 call()
 
 
